@@ -39,6 +39,8 @@ extern "C" {
 #define SKV_KV_F16 0
 #define SKV_KV_I8 1
 #define SKV_KV_E4M3 2
+/* Keys and values in 4 bits: page records of 16 tokens, [num_pages, Hkv, 18, D] bytes (skv_gqa_decode_kv4). */
+#define SKV_KV_INT4 3
 /* OR-ed into kv_dtype of skv_gqa_decode_paged: the output tensor holds bf16 instead of fp16 elements. */
 #define SKV_OUT_BF16 0x100
 /* OR-ed into kv_dtype of skv_gqa_decode_paged, skv_quest_decode and skv_rope_quant_append: mixed-precision pages.  K stays 8-bit
@@ -201,6 +203,71 @@ int skv_rope_quant_append(const void* qkv, int qkv_is_bf16, void* q_out, void* k
                           long long scale_stride_page, long long scale_stride_head,
                           float rope_theta, void* meta, int meta_block_size, int meta_num_blocks,
                           int num_pages, int* status, int device, void* stream);
+
+/* ---- rotary positions ---------------------------------------------------------------
+ * No reference counterpart (the reference calls Hugging Face's rotary module, benchmarks/llama_integration_benchmark.py
+ * :152-160).  For every token t and pair i < rotary_dim / 2 of every head of q [T, Hq, D] and k [T, Hk, D]:
+ *   (x, y) -> rope_factor * (x cos a - y sin a, y cos a + x sin a),  a = positions[t] * f_i (adjoint = 1: -a, the gradient)
+ * with the pair in channels (i, i + rotary_dim / 2) or, interleaved = 1, (2i, 2i + 1); channels from rotary_dim on are
+ * copied.  freqs: device array of rotary_dim / 2 uint64, round(f_i / (2 pi) * 2^64): the angle at any position is exact to
+ * the rounding of f_i.  dtype: 0 fp16, 1 bf16, 2 fp32 (q, k and outputs alike; arithmetic in fp32).  positions: int32, or
+ * int64 with positions_are_64.  Strides in elements, channels contiguous; an output may be its input (then channels
+ * behind rotary_dim are not touched), not overlap it otherwise.  Hq or Hk may be 0 with null pointers.  rotary_dim even. */
+int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* positions,
+               int positions_are_64, const unsigned long long* freqs, int T, int Hq, int Hk, int D,
+               int rotary_dim, int interleaved, float rope_factor, int adjoint,
+               long long q_stride_t, long long q_stride_h, long long k_stride_t, long long k_stride_h,
+               long long q_out_stride_t, long long q_out_stride_h, long long k_out_stride_t,
+               long long k_out_stride_h, int device, void* stream);
+
+/* ---- tokens into and out of a paged cache, any number per sequence ------------------
+ * No reference counterpart (its cache update is DynamicCache.update, benchmarks/llama_integration_benchmark.py:173).
+ * skv_append_tokens: row t of qkv ([T, >= (Hq + 2 Hkv) * D] fp16 or bf16, qkv_stride elements between rows: q heads, k
+ *   heads, v heads) belongs to the sequence b with cu_new[b] <= t < cu_new[b + 1] (cu_new: int32 [B + 1]; NULL: row b to
+ *   sequence b, T = B) and takes position seq_lens[b] + t - cu_new[b] of it.  q and k are rotated as by skv_rotary
+ *   (rope_freqs NULL: not at all) at that position, or at positions[t] when given; q goes to q_out [T, Hq, D] (fp16, or
+ *   bf16 with q_out_is_bf16), k and v are quantised and stored.  Rows behind cu_new[B] are left alone, in q_out too.
+ *   seq_lens is not modified.  A position past max_pages * page_size stores nothing, nor does one whose page-table entry
+ *   lies outside [0, num_pages), which sets SKV_DEV_BAD_PAGE in *status (optional).  A row (4-bit: a group of 32
+ *   channels) that is not finite is stored with scale NaN.  rotary_dim is a multiple of 16 (interleaved: of 8).
+ * skv_read_tokens: row t with cu[b] <= t < cu[b + 1] receives the token at position starts[b] + t - cu[b] (starts NULL: 0)
+ *   of sequence b as values, k_out / v_out [T, Hkv, D] fp16 (bf16 with out_is_bf16), code * scale rounded once; zeros where
+ *   the cache has no page.  Rows behind cu[B] are left alone.
+ * Caches (kv_dtype): SKV_KV_I8 or SKV_KV_E4M3, with SKV_V_INT4 for 4-bit values, pools and strides as for
+ *   skv_rope_quant_append (D = 128, rows 16-byte aligned); SKV_KV_INT4: k_pool = base of the records, strides of page and
+ *   head in bytes, the other pool arguments unused (D = 64 or 128, page_size 16). */
+int skv_append_tokens(const void* qkv, int qkv_is_bf16, long long qkv_stride, void* q_out, int q_out_is_bf16,
+                      const unsigned long long* rope_freqs, int rotary_dim, int interleaved, float rope_factor,
+                      const void* positions, int positions_are_64, const int* cu_new, const int* page_table,
+                      const int* seq_lens, void* k_pool, void* v_pool, float* k_scale_pool, float* v_scale_pool, int T, int B,
+                      int Hq, int Hkv, int D, int kv_dtype, int page_size, int max_pages, int num_pages,
+                      long long pool_stride_page, long long pool_stride_head, long long pool_stride_slot,
+                      long long scale_stride_page, long long scale_stride_head, int* status, int device, void* stream);
+int skv_read_tokens(const void* k_pool, const void* v_pool, const float* k_scale_pool, const float* v_scale_pool,
+                    const int* page_table, const int* cu, const int* starts, void* k_out, void* v_out, int out_is_bf16, int T,
+                    int B, int Hkv, int D, int kv_dtype, int page_size, int max_pages, int num_pages,
+                    long long pool_stride_page, long long pool_stride_head, long long pool_stride_slot,
+                    long long scale_stride_page, long long scale_stride_head, int* status, int device, void* stream);
+
+/* ---- dense GQA decode over a paged cache held in 4 bits -----------------------------
+ * No reference counterpart.  Keys and values in page records of 16 tokens, 18 * D bytes per (page, head): 8 D bytes of key
+ * codes, 8 D of value codes, 2 D of scales.  Every 32 channels of a row share a bf16 scale = bf16(amax / 7) (0 for zeros,
+ * NaN for a group that is not finite), code = clamp(rne(x / scale), -7, 7) in the nibble code + 8, even nibble low.  Token
+ * t = 4i + 2j + e of a page has place 8j + 2i + e:
+ *   keys    byte place * D/2 + c * D/8 + 4w + n/2                    channel 32w + 8c + n  (c < 4, n < 8)
+ *   values  byte 8D + j * 4D + g * D/2 + i * D/8 + e * D/16 + 2w + n/2   channel 32w + 4g + n  (g < 8, n < 4)
+ *   scales  bf16 element at byte 16D + place * D/8 + 2w (keys), + D/16 (values), group w < D/32
+ * q, out: [T, Hq, D], fp16 or bf16 each.  cu_q int32 [B + 1]: rows cu_q[b] .. cu_q[b + 1] are the last query tokens of
+ * sequence b, query i of n sees positions < seq_lens[b] - n + i + 1 (none: zeros); NULL: one query per sequence, T = B.
+ * Rows behind cu_q[B] of out are left alone.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
+ * skv_gqa_decode_paged.  pool strides in bytes.  D = 64 or 128, any Hq / Hkv.  The result does not depend on timing.
+ * Workspace: skv_gqa_decode_kv4_workspace_bytes(D), status word at offset 0; its first 8192 bytes are zero before the
+ * first use and left reusable. */
+size_t skv_gqa_decode_kv4_workspace_bytes(int D);
+int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int* page_table, const int* seq_lens,
+                       const int* cu_q, void* out, int out_is_bf16, void* workspace, size_t workspace_bytes, int T, int B, int N,
+                       int Hq, int Hkv, int D, int max_pages, int num_pages, long long pool_stride_page,
+                       long long pool_stride_head, float scale, int device, void* stream);
 
 /* ---- token-sparse decode ----------------------------------------------------------
  * Replaces kv_evict_quant_forward(Q, K, V, top_k, use_int8=false)  (csrc/kernels/kv_evict_quant.cu:272-364,

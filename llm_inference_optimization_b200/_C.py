@@ -252,3 +252,56 @@ def fused_gqa_paged(Q: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, 
         float(scale), dev, stream)
     _lib.check(rc, "fused_gqa_paged")
     return out
+
+
+def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: Tensor | None, scale: float, *,
+                  cu_q: Tensor | None = None, max_seq_len: int | None = None, out: Tensor | None = None) -> Tensor:
+    """Dense GQA attention over a paged cache whose keys and values are held in 4 bits (``skv_gqa_decode_kv4``).
+
+    Q ``[T,Hq,D]`` fp16 or bf16, D 64 or 128; ``pool`` uint8 ``[num_pages,Hkv,18,D]`` page records of 16 tokens
+    (``paged.PagedKV4``; the first two dimensions may be strided); ``page_table`` int32 ``[B,max_pages]`` (``None``:
+    sequence b owns pages ``b*max_pages ...``); ``seq_lens`` int32 ``[B]`` (``None``: every sequence is full).  Without
+    ``cu_q`` row b is the one query of sequence b; with ``cu_q`` (int32 ``[B+1]``) rows ``cu_q[b]..cu_q[b+1]`` are the
+    last tokens of sequence b, each seeing the tokens up to itself -- drafted tokens, a chunk of prompt.  A query that
+    sees nothing gets zeros; rows behind ``cu_q[B]`` are not written.  Returns ``[T,Hq,D]`` in Q's dtype, or in that of
+    ``out`` (fp16 or bf16).  No reference counterpart.
+    """
+    _require(Q.is_cuda and Q.dtype in (torch.float16, torch.bfloat16) and Q.dim() == 3 and Q.is_contiguous(),
+             "Q must be a contiguous fp16 or bf16 CUDA tensor [T,Hq,D]")
+    T, Hq, D = Q.shape
+    dev = Q.device
+    _require(pool.dtype == torch.uint8 and pool.dim() == 4 and pool.shape[2] == 18 and pool.shape[3] == D and pool.device == dev
+             and pool.stride(3) == 1 and pool.stride(2) == D, "pool must be uint8 [num_pages,Hkv,18,D] page records on Q's device")
+    num_pages, Hkv = pool.shape[:2]
+    if page_table is not None:
+        _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
+                 and page_table.device == dev, "page_table must be a contiguous int32 [B,max_pages] tensor on Q's device")
+        B, max_pages = page_table.shape
+    else:
+        B = T if cu_q is None else cu_q.numel() - 1
+        _require(B > 0 and num_pages % B == 0, "without a page table num_pages must be B * max_pages")
+        max_pages = num_pages // B
+    if cu_q is None:
+        _require(T == B, "one query row per sequence, or cu_q")
+    else:
+        _require(cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous() and cu_q.device == dev,
+                 "cu_q must be a contiguous int32 [B+1] tensor on Q's device")
+    if seq_lens is not None:
+        _require(seq_lens.dtype == torch.int32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
+                 and seq_lens.device == dev, "seq_lens must be a contiguous int32 [B] tensor on Q's device")
+    N = int(max_seq_len) if max_seq_len is not None else max_pages * 16
+    _require(0 < N <= max_pages * 16, "max_seq_len must be in (0, max_pages * 16]")
+    if out is None:
+        out = torch.empty_like(Q)
+    else:
+        _require(out.dtype in (torch.float16, torch.bfloat16) and out.shape == Q.shape and out.is_contiguous()
+                 and out.device == dev, "out must be a contiguous fp16 or bf16 tensor of Q's shape on Q's device")
+    lib = _lib.load()
+    ws = _workspace.scratch("gqa_kv4", lib.skv_gqa_decode_kv4_workspace_bytes(D), 8192, dev)
+    rc = lib.skv_gqa_decode_kv4(
+        Q.data_ptr(), Q.dtype == torch.bfloat16, pool.data_ptr(), None if page_table is None else page_table.data_ptr(),
+        None if seq_lens is None else seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), out.data_ptr(),
+        out.dtype == torch.bfloat16, ws.data_ptr(), ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages,
+        pool.stride(0), pool.stride(1), float(scale), _dev_index(Q), torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "fused_gqa_kv4")
+    return out

@@ -14,7 +14,7 @@ import os
 # SKV_B200_LIB points the loader at another build of the same library (for example an instrumented one).
 LIB_PATH = Path(os.environ.get("SKV_B200_LIB") or Path(__file__).resolve().parent / "csrc" / "libskv_b200.so")
 
-KV_F16, KV_I8, KV_E4M3 = 0, 1, 2
+KV_F16, KV_I8, KV_E4M3, KV_INT4 = 0, 1, 2, 3
 QUANT_NONE, QUANT_INT8, QUANT_E4M3, QUANT_CAST = 0, 1, 2, 3
 ORDER_POSITION, ORDER_SCORE = 0, 1
 
@@ -69,6 +69,14 @@ SIGNATURES = {
     "skv_silu_mul": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "skv_rope_quant_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
                                    _ll, _ll, _ll, _ll, _ll, _f, _vp, _i, _i, _i, _vp, _i, _vp]),
+    "skv_rotary": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i,
+                        _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _i, _vp]),
+    "skv_append_tokens": (_i, [_vp, _i, _ll, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _i, _i, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _vp, _i, _vp]),
+    "skv_read_tokens": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+                             _ll, _ll, _ll, _ll, _ll, _vp, _i, _vp]),
+    "skv_gqa_decode_kv4_workspace_bytes": (_sz, [_i]),
+    "skv_gqa_decode_kv4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _f, _i, _vp]),
     "skv_gqa_decode_noalloc_status": (_i, [_i, _vp, C.POINTER(_i)]),
     "skv_gqa_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _vp, _f, _i, _vp]),
 }

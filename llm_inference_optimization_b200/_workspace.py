@@ -25,6 +25,18 @@ def get(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
     return buf
 
 
+def scratch(kind: str, nbytes: int, head: int, device: torch.device) -> torch.Tensor:
+    """Like :func:`get` for kernels of which only the first ``head`` bytes must be zero, and safe under graph capture.
+
+    A call that is being captured gets a buffer of the graph's own, whose head is cleared by a node of the graph: two
+    graphs, or a graph and eager calls, never share one, however their replays overlap."""
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:head].zero_()
+        return buf
+    return get(kind, nbytes, device)
+
+
 def all_of(kind: str, device: torch.device) -> list[torch.Tensor]:
     """Every cached workspace of one kind on a device (one per stream that has launched with it)."""
     index = device.index if device.index is not None else torch.cuda.current_device()

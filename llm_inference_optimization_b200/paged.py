@@ -221,6 +221,173 @@ def rope_quant_append(qkv: Tensor, kv: PagedKV, Hq: int, rope_theta: float, *, m
     return q
 
 
+@dataclass
+class PagedKV4:
+    """Paged cache whose keys and values are held in 4 bits: page records of 16 tokens, uint8 ``[num_pages, Hkv, 18, D]``
+    (D 64 or 128): 9 bytes for 8 channels of a key and a value against 16.5 in the 8-bit records.
+
+    Every 32 channels of a row share a bf16 scale ``amax / 7``.  The order of bytes inside a record is the attention
+    kernel's (``skv_gqa_decode_kv4`` in the header); :func:`pack_kv4` and :func:`unpack_kv4` convert.  Fill it with
+    :func:`append_tokens`.  A view of a larger buffer will do (for example one layer of ``[num_pages, layers, Hkv, 18, D]``)."""
+    buf: Tensor
+    page_table: Tensor | None   # int32 [B, max_pages]; None: sequence b owns pages b*max_pages ...
+    seq_lens: Tensor | None     # int32 [B]
+    batch: int
+
+    page_size = 16
+
+    @property
+    def head_dim(self) -> int:
+        return self.buf.shape[3]
+
+    @property
+    def max_pages(self) -> int:
+        return self.page_table.shape[1] if self.page_table is not None else self.buf.shape[0] // self.batch
+
+    @property
+    def capacity(self) -> int:
+        return self.max_pages * 16
+
+    def decode(self, Q: Tensor, scale: float, *, cu_q: Tensor | None = None, max_seq_len: int | None = None,
+               out: Tensor | None = None) -> Tensor:
+        """Dense GQA attention over the whole cache, one or several query tokens per sequence (``_C.fused_gqa_kv4``)."""
+        return _C.fused_gqa_kv4(Q, self.buf, self.page_table, self.seq_lens, scale, cu_q=cu_q, max_seq_len=max_seq_len, out=out)
+
+
+KV4_RECORD_ROWS = 18  # rows of D bytes per (page, head): 8 of key codes, 8 of value codes, 2 of bf16 scales
+
+
+def pack_kv4(k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor) -> Tensor:
+    """Codes in -7..7 (int8 ``[num_pages,Hkv,16,D]``) and their bf16 scales (``[num_pages,Hkv,16,D/32]``) as page records."""
+    P, H, S, D = k_codes.shape
+    W = D // 32
+    _C._require(S == 16 and D in (64, 128) and v_codes.shape == k_codes.shape and k_scale.shape == (P, H, 16, W)
+                and v_scale.shape == k_scale.shape and k_scale.dtype == torch.bfloat16 and v_scale.dtype == torch.bfloat16,
+                "4-bit page records hold [num_pages,Hkv,16,D] codes, D 64 or 128, and bf16 [num_pages,Hkv,16,D/32] scales")
+
+    def nibbles(c):
+        u = (c + 8).to(torch.uint8)
+        return u[..., 0::2] | (u[..., 1::2] << 4)
+
+    # tokens 4i + 2j + e; keys j i e c w n, values j g i e w n (see the header)
+    kb = nibbles(k_codes).view(P, H, 4, 2, 2, W, 4, 4).permute(0, 1, 3, 2, 4, 6, 5, 7).reshape(P, H, 8, D)
+    vb = nibbles(v_codes).view(P, H, 4, 2, 2, W, 8, 2).permute(0, 1, 3, 6, 2, 4, 5, 7).reshape(P, H, 8, D)
+    sc = torch.stack([k_scale, v_scale], 3).view(P, H, 4, 2, 2, 2, W).permute(0, 1, 3, 2, 4, 5, 6).contiguous()
+    return torch.cat([kb, vb, sc.view(torch.uint8).reshape(P, H, 2, D)], 2)
+
+
+def unpack_kv4(buf: Tensor):
+    """``(k_codes, k_scale, v_codes, v_scale)`` of page records: int8 codes and bf16 scales, the inverse of :func:`pack_kv4`."""
+    P, H, R, D = buf.shape
+    _C._require(R == KV4_RECORD_ROWS and D in (64, 128) and buf.dtype == torch.uint8, "not 4-bit page records")
+    W = D // 32
+
+    def codes(b):
+        return (torch.stack([b & 15, b >> 4], -1).flatten(-2).to(torch.int8) - 8)
+
+    k = codes(buf[:, :, :8].reshape(P, H, 2, 4, 2, 4, W, 4)).permute(0, 1, 3, 2, 4, 6, 5, 7).reshape(P, H, 16, D)
+    v = codes(buf[:, :, 8:16].reshape(P, H, 2, 8, 4, 2, W, 2)).permute(0, 1, 4, 2, 5, 6, 3, 7).reshape(P, H, 16, D)
+    sc = buf[:, :, 16:].contiguous().view(torch.bfloat16).reshape(P, H, 2, 4, 2, 2, W).permute(0, 1, 3, 2, 4, 5, 6)
+    sc = sc.reshape(P, H, 16, 2, W)
+    return k, sc[..., 0, :], v, sc[..., 1, :]
+
+
+def _token_cache(kv):
+    """Pool arguments of the append / read kernels, in their order, up to the strides; and (Hkv, D, device)."""
+    if isinstance(kv, PagedKV4):
+        b = kv.buf
+        _C._require(b.is_cuda and b.dtype == torch.uint8 and b.dim() == 4 and b.shape[2] == KV4_RECORD_ROWS and b.shape[3] in (64, 128)
+                    and b.stride(3) == 1 and b.stride(2) == b.shape[3], "not a cache of 4-bit page records")
+        _, Hkv, _, D = b.shape
+        pools, fmt, strides, pages = (b.data_ptr(), None, None, None), _lib.KV_INT4, (b.stride(0), b.stride(1), 0, 0, 0), b.shape[0]
+        dev, size = b.device, 16
+    else:
+        strides = _pool_args(kv)
+        pages, Hkv, size, D = kv.k_pool.shape
+        pools = (kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr())
+        fmt = _C._code_dtype(kv.k_pool) | (_C.SKV_V_INT4 if kv.v_bits == 4 else 0)
+        dev = kv.k_pool.device
+    t = kv.page_table
+    if t is not None:
+        _C._require(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == kv.batch and t.is_contiguous() and t.device == dev,
+                    "page_table must be a contiguous int32 [B,max_pages] tensor on the cache's device")
+    else:
+        _C._require(pages % kv.batch == 0, "without a page table num_pages must be B * max_pages")
+    return pools, fmt, (size, kv.max_pages, pages, *strides), Hkv, D, dev
+
+
+def _int32(t: Tensor, shape, dev, what: str) -> int:
+    _C._require(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous() and t.device == dev,
+                f"{what} must be a contiguous int32 {list(shape)} tensor on the cache's device")
+    return t.data_ptr()
+
+
+def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, cu_new: Tensor | None = None,
+                  positions: Tensor | None = None, q_out: Tensor | None = None, status: Tensor | None = None) -> Tensor:
+    """Rotate, quantise and store any number of new tokens per sequence: a prompt, a chunk of one, drafted tokens, a step.
+
+    ``qkv`` ``[T, (Hq + 2*Hkv) * D]`` fp16 or bf16 (fused projection output; rows may be strided).  Rows
+    ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``; ``None``: one row per sequence) are the next tokens of sequence b and take
+    positions ``kv.seq_lens[b]``, ``+ 1``, ...; ``seq_lens`` is read, not advanced.  ``rope`` (a ``RotaryEmbedding``;
+    ``None``: no rotation) turns q and k at those positions, or at ``positions`` (int32 or int64 ``[T]``) where the place in
+    the cache is not the place in the text (an evicted, compacted cache).  Returns the rotated query ``[T, Hq, D]``: fp16, or
+    ``q_out`` (fp16 or bf16).  Rows behind ``cu_new[B]`` are left alone.  Tokens past a sequence's page list are not stored;
+    neither is one whose page-table entry lies outside the pool, which sets ``SKV_DEV_BAD_PAGE`` (2) in ``status`` (an
+    int32 device tensor of one element).  Serves ``PagedKV4`` (D 64 or 128) and every ``PagedKV`` (D 128); a rotary width
+    must be a multiple of 16 (interleaved: of 8).  Block metadata is not kept current: rebuild it (``build_block_meta``).
+    """
+    pools, fmt, geometry, Hkv, D, dev = _token_cache(kv)
+    _C._require(qkv.device == dev and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype in (torch.float16, torch.bfloat16)
+                and Hq >= 0 and qkv.shape[1] == (Hq + 2 * Hkv) * D,
+                "qkv must be fp16/bf16 [T,(Hq+2Hkv)*D] on the cache's device, channels contiguous")
+    T, B = qkv.shape[0], kv.batch
+    _C._require(kv.seq_lens is not None, "the cache needs seq_lens")
+    lens = _int32(kv.seq_lens, (B,), dev, "seq_lens")
+    if cu_new is None:
+        _C._require(T == B, "one row per sequence, or cu_new")
+    freqs, width, inter, factor = (None, 0, 0, 1.0) if rope is None else rope.kernel_args(D, dev)
+    if positions is not None:
+        _C._require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (T,) and positions.is_contiguous()
+                    and positions.device == dev, "positions must be a contiguous int32 or int64 [T] tensor on the cache's device")
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=dev)
+    else:
+        _C._require(q_out.dtype in (torch.float16, torch.bfloat16) and q_out.shape == (T, Hq, D) and q_out.is_contiguous()
+                    and q_out.device == dev, "q_out must be a contiguous fp16 or bf16 [T,Hq,D] tensor on the cache's device")
+    rc = _lib.load().skv_append_tokens(
+        qkv.data_ptr(), qkv.dtype == torch.bfloat16, qkv.stride(0) if T > 1 else qkv.shape[1], q_out.data_ptr(),
+        q_out.dtype == torch.bfloat16, freqs, width, inter, factor, None if positions is None else positions.data_ptr(),
+        positions is not None and positions.dtype == torch.int64,
+        None if cu_new is None else _int32(cu_new, (B + 1,), dev, "cu_new"),
+        None if kv.page_table is None else kv.page_table.data_ptr(), lens, *pools, T, B, Hq, Hkv, D, fmt, *geometry,
+        None if status is None else _int32(status, (1,), dev, "status"), _C._dev_index(qkv),
+        torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "append_tokens")
+    return q_out
+
+
+def read_tokens(kv: "PagedKV | PagedKV4", cu: Tensor, rows: int, *, starts: Tensor | None = None,
+                dtype: torch.dtype = torch.float16, status: Tensor | None = None):
+    """Rows of cached tokens as values: ``(K, V)`` ``[rows, Hkv, D]`` fp16 or bf16, code times scale rounded once.
+
+    Rows ``cu[b]..cu[b+1]`` (int32 ``[B+1]``, ``cu[B] <= rows``) are positions ``starts[b]``, ``+ 1``, ... (int32 ``[B]``;
+    ``None``: from 0) of sequence b: the prefix that a chunk of prompt attends to through another kernel, or a check of what
+    was stored.  ``kv.seq_lens`` is not consulted.  Rows behind ``cu[B]`` are not written; a position without a page reads as
+    zeros (``status`` as in :func:`append_tokens`)."""
+    pools, fmt, geometry, Hkv, D, dev = _token_cache(kv)
+    _C._require(dtype in (torch.float16, torch.bfloat16) and rows >= 0, "read_tokens returns fp16 or bf16 rows")
+    B = kv.batch
+    K = torch.empty((rows, Hkv, D), dtype=dtype, device=dev)
+    V = torch.empty_like(K)
+    rc = _lib.load().skv_read_tokens(
+        *pools, None if kv.page_table is None else kv.page_table.data_ptr(), _int32(cu, (B + 1,), dev, "cu"),
+        None if starts is None else _int32(starts, (B,), dev, "starts"), K.data_ptr(), V.data_ptr(), dtype == torch.bfloat16,
+        rows, B, Hkv, D, fmt, *geometry, None if status is None else _int32(status, (1,), dev, "status"), _C._dev_index(K),
+        torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "read_tokens")
+    return K, V
+
+
 def repage_evicted(res, *, pool: Tensor | None = None, page_ids: Tensor | None = None) -> PagedKV:
     """Put the compacted, quantised output of ``fused_kv_evict`` back into paged form (page reclamation).
 
