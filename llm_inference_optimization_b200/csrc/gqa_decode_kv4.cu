@@ -14,15 +14,16 @@
 //     (bits 4-7), subnormal and exact, and products with it are exact in the fp32 accumulator: 5 logic operations for 8
 //     codes.  The factor 16 between the two kinds is put into the query (its own exponent is normalised first) and, for
 //     values, divided out of the rows of O at the end.  Codes are u - 8: the 8 is taken out of the scores by starting the
-//     accumulators at -8 sum(q) and out of O with sum(p), which one product with a tile of ones per group yields.
+//     accumulators at -8 ks sum(q), a small product of its own, and out of the value codes by an exact packed addition.
 //   * ks multiplies the fp32 partial scores of its group; vs is folded into the weights before they are rounded to fp16.
-//     So that neither small nor large value scales under- or overflow there, the running maximum is taken over
-//     s + (a bound of log2 vs), and the weights, at most 1, carry a factor 2^14.  (One rounding to 11 bits per weight.)
+//     (One rounding to 11 bits per weight.)  The reference that scores are taken against before exp2 only has to keep the
+//     weights within fp16: it follows the running maximum of scores and value scales in jumps of several powers of two, so
+//     a record costs one vote where an exact running maximum costs shuffles and a rescaling of O.
 //   * Tokens on the M side of both products (S^T = K Q^T, O^T = V^T P^T), up to 8 NT columns (query token, head) on the
 //     N side; P goes from the one layout to the other by movmatrix.
 //
 // Streaming: every warp is on its own -- it copies records to a ring of its own with cp.async (16 bytes per lane and
-// request: a record is five requests of a warp), keeps its own softmax state, and meets the others only at the end of a
+// request: two records are nine requests of a warp), keeps its own softmax state, and meets the others only at the end of a
 // segment.  No producer warps and no barriers in the loop.
 //
 // Work split: the host does not know the lengths.  Work is counted in records over (kv-head, sequence, chunk of columns)
@@ -37,31 +38,40 @@
 namespace skv {
 namespace kv4 {
 
-constexpr int NW = 8;                 // warps per CTA
-constexpr int THREADS = NW * 32;
+// Weights are kept below 2^WEIGHT_MAX (fp16 holds 2^15.99) and are at most 2^WEIGHT_AIM when their reference has just moved:
+// four powers of two before it moves again, and eleven bits for every weight down to 2^-24 of the largest.
+constexpr float WEIGHT_MAX = 14.f, WEIGHT_AIM = 10.f;
+constexpr float NOTHING = -1e30f;     // reference of a column that has seen no token
+constexpr int SETUP = 48;          // what starting an item costs a CTA, in records: query, first loads, merge
 constexpr int MIN_UNITS = 16;         // records per CTA at least: shorter runs are all start and end
 constexpr size_t TICKET_OFF = 256, PARTIAL_OFF = 8192;
 constexpr int MAX_GRID = 320;         // CTAs of one wave (a combine keeps this many (max, sum) pairs in registers)
 static_assert(MAX_GRID * 4 <= PARTIAL_OFF - TICKET_OFF, "tickets");
 
 template <int D, int NT> struct Shape {
+    static constexpr int NW = NT == 1 ? 6 : 8;           // warps per CTA: as many as the registers allow
+    static constexpr int THREADS = NW * 32;
     static constexpr int W = D / 32;                     // scale groups per row
     static constexpr int REC = kv4_record_bytes<D>();
-    static constexpr int STAGES = NT == 1 ? 4 : 5;
+    static constexpr int STAGES = 5;
     static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
     static constexpr int ROW = D + 4;                    // merge rows, padded: 16-byte stores of a warp spread over the banks
     static constexpr int RING = NW * STAGES * REC;
-    static constexpr int MERGE = NW * 8 * ROW * 4;       // one n-tile (8 columns) at a time
+    static constexpr int MAX_N = MAX_GRID / (NT == 1 ? 1 : 2);                     // partial results of an item
+    static constexpr int SCRATCH = MAX_N * 8 * NT * 4 + 16 * 4 + THREADS * 16 + 16;   // what combine() needs
+    static constexpr int TILE = NW * 8 * ROW * 4;        // one n-tile (8 columns) of every warp
+    static constexpr int MERGE = TILE > SCRATCH ? TILE : SCRATCH;
     static constexpr int ML = NW * 8 * NT * 8;           // (max, sum) per warp and column
-    static constexpr size_t SMEM = RING + MERGE + ML + 16;
-    static_assert(MAX_GRID / (NT == 1 ? 1 : 2) * 8 * NT * 4 + 16 * 4 + THREADS * 16 + 16 <= MERGE, "combine's scratch");
+    static constexpr int QUERY = NT * (W * 512 + 32 * 12);   // the item's columns as operands, and 12 bytes per lane
+    static constexpr size_t SMEM = RING + MERGE + ML + 2 * QUERY + 128;
 };
 
 struct Params {
     const void* q;
     void* out;
     const uint8_t* pool;
-    long long sp, sh;            // record strides in bytes: page, head
+    uint32_t sp;                 // record strides in bytes: page (below 4 GB: one multiply-add makes an address), head
+    long long sh;
     const int* page_table;       // null: page = b * max_pages + i
     const int* seq_lens;         // null: N
     const int* cu_q;             // null: one query token per sequence
@@ -95,11 +105,38 @@ struct Segment {
     int c_first, c_last;         // CTAs that share it, else
 };
 
-__device__ __forceinline__ void mma_f16_c(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+// products that start from zero
+__device__ __forceinline__ void mma_f16_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// -136 and -128 times 2^-24, twice: what a byte of value codes, and its upper nibble in place, hold too much
+constexpr uint32_t MINUS_136 = 0x80888088u, MINUS_128 = 0x80808080u;
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// cp.async, or zeros
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool p) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(p ? 16 : 0) : "memory");
+}
+// cp.async under a predicate, without a branch
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool p) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}"
+                 ::"r"(dst), "l"(src), "r"((int)p) : "memory");
 }
 
 template <int BYTES>
@@ -116,14 +153,7 @@ __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 
 template <int N> __device__ __forceinline__ float group_scale(const uint32_t (&s)[N], int first, int w) {
     return (w & 1) ? bf_hi(s[first + (w >> 1)]) : bf_lo(s[first + (w >> 1)]);
 }
-// e with max(vs) < 2^e, within what keeps the sums of weights in range
-template <int D> __device__ __forceinline__ float scale_bound(const uint32_t (&s)[D / 32]) {
-    uint32_t m = s[D / 64];
-    if (D == 128) m = __vmaxu2(m, s[D / 64 + 1]);
-    m = max(m & 0x7fff0000u, (m << 16) & 0x7fff0000u);
-    const float e = __uint_as_float((m >> 23) | 0x4b000000u) - (8388608.f + 126.f);   // exponent field -> float
-    return fminf(fmaxf(e, -60.f), 100.f);
-}
+template <bool V> struct Constant { static constexpr bool value = V; };
 
 // Column `col` of the item's list (query token col / G, head col % G), channels d .. d + 3
 __device__ __forceinline__ void store_out(const Params& p, const Segment& x, int D, int col, int d, float4 v, float L) {
@@ -141,14 +171,29 @@ __device__ __forceinline__ void store_out(const Params& p, const Segment& x, int
 
 // Sum of an item's n partial results, by the whole CTA.  scratch: n * cols weights, 16 floats, THREADS * 4 floats.  The
 // threads are split over the partials where the columns leave them free; every sum has one order, whoever runs it.
-template <int D, int NC>
+template <int D, int NC, int THREADS>
 __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n, int cols, int col0, float* scratch) {
-    constexpr int REGS = (MAX_GRID + 31) / 32;
+    constexpr int REGS = (MAX_GRID / (NC / 8) + 31) / 32;
+    constexpr int NW = THREADS / 32;
+    constexpr int U = 12;                               // partial rows in flight per thread
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* weight = scratch;                            // [n][cols]
     float* sums = scratch + ((n * cols + 3) & ~3);      // [cols]
     float4* part = reinterpret_cast<float4*>(sums + 16);
-    auto slot = [&](int i) { return 2ll * (x.c_first + i) + (i == 0 ? 1 : 0); };
+    const int places = cols * (D / 4);
+    const int subs = max(1, THREADS / places);
+    // the k-th partial row of thread i: the same for all but the first CTA, whose slot is its second
+    auto row = [&](int i, int k) {
+        const int pos = i % places;
+        const long long slot = 2ll * (x.c_first + k) + (k == 0 ? 1 : 0);
+        return p.partial_o + (slot * NC + pos / (D / 4)) * D + pos % (D / 4) * 4;
+    };
+    float4 v[U];                                        // asked for before the weights are known (past the end: the last row again)
+    if (threadIdx.x < places * subs) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = __ldcg(reinterpret_cast<const float4*>(row(threadIdx.x, min(threadIdx.x / places + u * subs, n - 1))));
+    }
     for (int c = warp; c < cols; c += NW) {
         float2 ml[REGS];
         float M = -INFINITY;
@@ -156,18 +201,17 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
         for (int i = 0; i < REGS; ++i) {
             const int k = lane + 32 * i;
             ml[i] = make_float2(-INFINITY, 0.f);
-            if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + (slot(k) * NC + c) * 2));
+            if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + ((2ll * (x.c_first + k) + (k == 0 ? 1 : 0)) * NC + c) * 2));
         }
 #pragma unroll
         for (int i = 0; i < REGS; ++i) M = fmaxf(M, ml[i].x);
         M = warp_max(M);
-        const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f;
 #pragma unroll
         for (int i = 0; i < REGS; ++i) {
             const int k = lane + 32 * i;
             if (k < n) {
-                const float w = fast_exp2(ml[i].x - ref);
+                const float w = fast_exp2(ml[i].x - M);
                 weight[k * cols + c] = w;
                 L = fmaf(ml[i].y, w, L);
             }
@@ -176,29 +220,26 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
         if (lane == 0) sums[c] = L;
     }
     __syncthreads();
-    const int places = cols * (D / 4);
-    const int subs = max(1, THREADS / places);
-    constexpr int U = 8;                                // partial rows in flight per thread
-    for (int i0 = threadIdx.x; i0 < places * subs; i0 += THREADS) {
-        const int sub = i0 / places, pos = i0 - sub * places;
-        const int c = pos / (D / 4), d = pos % (D / 4) * 4;
+    for (int i = threadIdx.x; i < places * subs; i += THREADS) {
+        const int sub = i / places, c = i % places / (D / 4);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k0 = sub; k0 < n; k0 += U * subs) {
-            float4 v[U];
+            if (i != threadIdx.x || k0 != sub) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)                 // (past the end: the last row again, with weight zero)
-                v[u] = __ldcg(reinterpret_cast<const float4*>(p.partial_o + (slot(min(k0 + u * subs, n - 1)) * NC + c) * D + d));
+                for (int u = 0; u < U; ++u) v[u] = __ldcg(reinterpret_cast<const float4*>(row(i, min(k0 + u * subs, n - 1))));
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int k = k0 + u * subs;
-                if (k >= n) break;
-                const float w = weight[k * cols + c];
-                acc.x = fmaf(v[u].x, w, acc.x); acc.y = fmaf(v[u].y, w, acc.y);
-                acc.z = fmaf(v[u].z, w, acc.z); acc.w = fmaf(v[u].w, w, acc.w);
+                const float w = k < n ? weight[k * cols + c] : 0.f;
+                if (k < n) {
+                    acc.x = fmaf(v[u].x, w, acc.x); acc.y = fmaf(v[u].y, w, acc.y);
+                    acc.z = fmaf(v[u].z, w, acc.z); acc.w = fmaf(v[u].w, w, acc.w);
+                }
             }
         }
-        if (subs == 1) store_out(p, x, D, col0 + c, d, acc, sums[c]);
-        else part[i0] = acc;
+        if (subs == 1) store_out(p, x, D, col0 + c, i % (D / 4) * 4, acc, sums[c]);
+        else part[i] = acc;
     }
     if (subs > 1) {
         __syncthreads();
@@ -215,134 +256,163 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_decode_kv4_kernel(const Params p) {
+__global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_PER_SM)) gqa_decode_kv4_kernel(const Params p) {
     using S = Shape<D, NT>;
-    constexpr int W = S::W, NC = 8 * NT, REC = S::REC, STAGES = S::STAGES;
+    constexpr int W = S::W, NC = 8 * NT, REC = S::REC, STAGES = S::STAGES, NW = S::NW, THREADS = S::THREADS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;
     extern __shared__ __align__(16) uint8_t smem[];
     float* merge = reinterpret_cast<float*>(smem + S::RING);
     float2* merge_ml = reinterpret_cast<float2*>(smem + S::RING + S::MERGE);       // [NW][NC]
-    int* flag = reinterpret_cast<int*>(smem + S::RING + S::MERGE + S::ML);
+    uint8_t* query = smem + S::RING + S::MERGE + S::ML;                             // two of them, for items in turn
+    // What only the change from one item to the next needs lives in shared memory: the loop below needs the registers.
+    struct State {
+        Segment sg;
+        int last;
+        long long at, end, run;                       // list position behind sg, end of this CTA's run, length of a run
+    };
+    static_assert(sizeof(State) <= 128, "state");
+    State* state = reinterpret_cast<State*>(query + 2 * S::QUERY);
     const uint32_t ring = smem_u32(smem) + warp * (STAGES * REC);
 
     pdl_wait_prior_grids();
     pdl_launch_dependents();
 
-    // ---- this CTA's run of the work list (every warp finds it for itself)
+    // ---- this CTA's run of the work list (every warp finds it for itself).  An item counts SETUP units for starting it and
+    // one for each record; positions fit 32 bits but for work of days, whose runs are found in 64.
     long long per_head = 0;
     for (int b = lane; b < p.B; b += 32) {
         const Seq s = sequence<NC>(p, b);
-        per_head += (long long)s.chunks * s.recs;
+        per_head += (long long)s.chunks * (SETUP + s.recs);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, o);
     const long long total = per_head * p.Hkv;
-    const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_UNITS);
-    long long at = run * blockIdx.x;                  // position in the list
-    const long long end = min(at + run, total);
-    if (at >= end) return;
-
-    Segment sg;
-    sg.h = (int)(at / per_head);
-    long long rest = at - sg.h * per_head;
-    sg.b = -1;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {            // find the sequence: a warp-wide prefix sum of 32 at a time
-        long long mine = 0;
-        if (b0 + lane < p.B) {
-            const Seq s = sequence<NC>(p, b0 + lane);
-            mine = (long long)s.chunks * s.recs;
-        }
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            sg.b = b0 + l;
-            rest -= __shfl_sync(0xffffffffu, upto - mine, l);
-            break;
-        }
-        rest -= __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (sg.b < 0) return;                             // (only if the lengths changed under the kernel)
-    sg.s = sequence<NC>(p, sg.b);
-    sg.chunk = (int)(rest / sg.s.recs);
-    sg.r0 = (int)(rest - (long long)sg.chunk * sg.s.recs);
-
-    auto finish_segment = [&]() {                     // r1 and who shares the item, from (b, chunk, r0) at list position `at`
-        sg.r1 = (int)min((long long)sg.s.recs, sg.r0 + (end - at));
+    const bool small = total < 0x40000000ll;
+    auto divide = [&](long long a, long long b) { return small ? (long long)((uint32_t)a / (uint32_t)b) : a / b; };
+    // the item at (h, b, chunk) of sg, from `place` on (its position in the item: SETUP + record), at list position `at`, which
+    // moves behind what is taken: false if the run ends before the first record
+    auto take = [&](Segment& sg, long long& at, int place, long long end, long long run) {
+        sg.r0 = max(place - SETUP, 0);
+        const long long stop = min((long long)(SETUP + sg.s.recs), place + (end - at));
+        sg.r1 = (int)max(stop - SETUP, 0ll);
         sg.whole = sg.r0 == 0 && sg.r1 == sg.s.recs;
         sg.c_first = sg.c_last = blockIdx.x;
-        if (!sg.whole) {
-            sg.c_first = (int)((at - sg.r0) / run);
-            sg.c_last = (int)((at - sg.r0 + sg.s.recs - 1) / run);
+        if (!sg.whole) {                              // the CTAs that hold its first and last record
+            sg.c_first = (int)divide(at - place + SETUP, run);
+            sg.c_last = (int)divide(at - place + SETUP + sg.s.recs - 1, run);
         }
+        at += stop - place;
+        return sg.r1 > sg.r0;
     };
-    finish_segment();
 
-    // ---- streaming: this warp's records of a segment are r0 + warp, r0 + warp + NW, ...
-    int n_rec = 0, page_now = 0, page_next = 0;
+    Segment first;
+    {
+        const long long run = max(divide(total + gridDim.x - 1, gridDim.x), (long long)MIN_UNITS);
+        long long at = run * blockIdx.x;
+        const long long end = min(at + run, total);
+        if (at >= end) return;
+        Segment& sg = first;
+        sg.h = (int)divide(at, per_head);
+        long long rest = at - sg.h * per_head;
+        sg.b = -1;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {        // find the sequence: a warp-wide prefix sum of 32 at a time
+            long long mine = 0;
+            if (b0 + lane < p.B) {
+                const Seq s = sequence<NC>(p, b0 + lane);
+                mine = (long long)s.chunks * (SETUP + s.recs);
+            }
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                sg.b = b0 + l;
+                rest -= __shfl_sync(0xffffffffu, upto - mine, l);
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (sg.b < 0) return;                         // (only if the lengths changed under the kernel)
+        sg.s = sequence<NC>(p, sg.b);
+        sg.chunk = (int)divide(rest, SETUP + sg.s.recs);
+        const int place = (int)(rest - (long long)sg.chunk * (SETUP + sg.s.recs));
+        if (!take(sg, at, place, end, run)) return;   // (a run that ends inside its first item's setup holds nothing)
+        if (threadIdx.x == 0) { state->sg = sg; state->at = at; state->end = end; state->run = run; }
+    }
+
+    // ---- streaming: this warp's k-th record of a segment is r_first + k NW
+    int n_rec = 0, rec_end = 0, r_first = 0, seq = 0;   // records of this warp; end of the records read; its first one; sequence
+    int in_off = 0;                                   // ring offset of the next copy
+    int page_now = 0, page_next = 0;
+    const uint8_t* head_base = nullptr;               // this lane's 16 bytes of the kv-head's record in page 0
     bool bad_page = false;
-    auto load_page = [&](const Segment& x, int k) {   // page of this warp's k-th record
-        const int r = x.r0 + warp + k * NW;
+    auto load_page = [&](int r) {
         int page = 0;
-        if (k < n_rec)
-            page = p.page_table ? __ldg(p.page_table + (long long)x.b * p.max_pages + r) : x.b * p.max_pages + r;
+        if (r < rec_end)
+            page = p.page_table ? __ldg(p.page_table + (long long)seq * p.max_pages + r) : seq * p.max_pages + r;
         return checked_page(page, p.num_pages, bad_page);
     };
-    auto issue = [&](const Segment& x, int k) {
+    auto issue = [&](int k) {
         if ((k & 31) == 0) {                          // pages of the next 32 records, one per lane, fetched 32 ahead
-            page_now = k ? page_next : load_page(x, lane);
-            page_next = load_page(x, k + 32 + lane);
+            const int r = r_first + (k + lane) * NW;
+            page_now = k ? page_next : load_page(r);
+            page_next = load_page(r + 32 * NW);
         }
         const int page = __shfl_sync(0xffffffffu, page_now, k & 31);
         if (k < n_rec) {
-            const uint8_t* src = p.pool + SKV_INDEX(page, p.num_pages) * p.sp + x.h * p.sh + lane * 16;
-            const uint32_t dst = ring + (k % STAGES) * REC + lane * 16;
+            const uint8_t* src = head_base + (unsigned long long)(uint32_t)SKV_INDEX(page, p.num_pages) * p.sp;
+            const uint32_t dst = ring + in_off + lane * 16;
 #pragma unroll
             for (int i = 0; i < REC / 512; ++i) cp_async16(dst + i * 512, src + i * 512);
-            if (lane < REC % 512 / 16) cp_async16(dst + REC / 512 * 512, src + REC / 512 * 512);
+            cp_async16_if(dst + REC / 512 * 512, src + REC / 512 * 512, lane < REC % 512 / 16);
         }
         cp_async_commit();
+        in_off = in_off == (STAGES - 1) * REC ? 0 : in_off + REC;
     };
-    // the last token that any column of the item sees bounds the records that are read
-    auto records = [&](const Segment& x) {
-        const int cols = x.s.nq * p.G;
-        const int i_last = (min(cols, (x.chunk + 1) * NC) - 1) / p.G;
+    // first copies of a segment, its query rows (as they are, to where the operands made of them will lie) ahead of the records
+    auto begin = [&](const Segment& x, uint8_t* q_to) {
+        const int total_cols = x.s.nq * p.G;
+        if (warp < NT) {
+            const int c = x.chunk * NC + warp * 8 + g;
+            const bool in = c < total_cols;
+            const long long row = in ? ((long long)(x.s.q0 + c / p.G) * p.Hq + x.h * p.G + c % p.G) * D : 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                cp_async16_or_zero(smem_u32(q_to) + ((warp * W + w) * 32 + lane) * 16, static_cast<const __half*>(p.q) + row + w * 32 + tq * 8, in);
+        }
+        // the last token that any column of the item sees bounds the records that are read
+        const int i_last = (min(total_cols, (x.chunk + 1) * NC) - 1) / p.G;
         const int seen = max(0, x.s.len - x.s.nq + i_last + 1);
-        const int r1 = min(x.r1, (seen + 15) >> 4);
-        return max(0, (r1 - x.r0 - warp + NW - 1) / NW);
-    };
-    auto begin = [&](const Segment& x) {
-        n_rec = records(x);
+        seq = x.b;
+        rec_end = min(x.r1, (seen + 15) >> 4);
+        r_first = x.r0 + warp;
+        n_rec = max(0, (rec_end - r_first + NW - 1) / NW);
+        in_off = 0;
+        head_base = p.pool + x.h * p.sh + lane * 16;
 #pragma unroll
-        for (int k = 0; k < STAGES - 1; ++k) issue(x, k);
+        for (int k = 0; k < STAGES - 1; ++k) issue(k);
     };
-    begin(sg);
+    begin(first, query);
 
-    for (;;) {
-        // ---- query columns of this item
-        const int col0 = sg.chunk * NC;               // first column: query token col0 / G, head col0 % G of the group
-        const int cols = min(sg.s.nq * p.G - col0, NC);
-        uint32_t qb[NT][W][4];
-        float init[NT][W][2], factor[NT][2];
-        int limit[NT][2];                             // tokens that columns 2tq, 2tq + 1 see
-        int limit_min = sg.s.len - sg.s.nq + col0 / p.G + 1;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = nt * 8 + g;
-            const int qi = (col0 + c) / p.G, hj = (col0 + c) % p.G;
-            const long long row = ((long long)(sg.s.q0 + qi) * p.Hq + sg.h * p.G + hj) * D;
+    for (int item = 0;; ++item) {
+        // ---- query columns of this item, as operands in shared memory, made by one warp per n-tile: [n-tile][group][lane] 16
+        // bytes, then two words of the bias operand and the factor of column g per lane
+        uint8_t* q_here = query + (item & 1) * S::QUERY;
+        const uint32_t q_ops = smem_u32(q_here);
+        uint32_t* q_words = reinterpret_cast<uint32_t*>(q_here + NT * W * 512);       // [n-tile][3][32]
+        if (warp < NT) {
+            const int nt = warp;
+            cp_async_wait<STAGES - 2>();
             float x[W][8];
             float amax = 0.f;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-                if (c < cols) raw = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + row + w * 32 + tq * 8);
+                const uint4 raw = *reinterpret_cast<const uint4*>(q_here + ((nt * W + w) * 32 + lane) * 16);
                 if (p.q_bf16) {
                     const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -362,132 +432,201 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_deco
             float sum[W];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
+                uint32_t b[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {          // nibbles i and i + 4; even i are masked out of bits 0-3, odd out of 4-7
                     const float k = (i & 1) ? up : up * 16.f;
-                    qb[nt][w][i] = pack_half2(x[w][i] * k, x[w][i + 4] * k);
+                    b[i] = pack_half2(x[w][i] * k, x[w][i + 4] * k);
                 }
+                *reinterpret_cast<uint4*>(q_here + ((nt * W + w) * 32 + lane) * 16) = make_uint4(b[0], b[1], b[2], b[3]);
                 float a = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][w][i]));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[i]));
                     a += (f.x + f.y) * ((i & 1) ? 1.f : 0.0625f);
                 }
                 a += __shfl_xor_sync(0xffffffffu, a, 1);
                 a += __shfl_xor_sync(0xffffffffu, a, 2);
                 sum[w] = a * -7.62939453125e-06f;       // -8 * 2^-20
             }
-            const float f = p.scale_log2 * __uint_as_float((uint32_t)min(max(e + 137, 1), 254) << 23);   // 2^20 / up
+            // the bias of a column's scores, sum_w ks_w sum[w], is a product of its own over the groups, the sums split into three
+            // bf16 terms (24 bits): k index 2 tq + {0, 1} (+ 8) is group 2 (tq & 1) + {0, 1} (D = 64: {0, 1}) of term tq >> 1 (+ 2)
+            uint32_t term[3][W / 2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int from = (2 * tq + j) * 4;
-                factor[nt][j] = __shfl_sync(0xffffffffu, f, from);
+            for (int i = 0; i < 3; ++i)
 #pragma unroll
-                for (int w = 0; w < W; ++w) init[nt][w][j] = __shfl_sync(0xffffffffu, sum[w], from);
-                const int cj = nt * 8 + 2 * tq + j;
-                limit[nt][j] = cj < cols ? sg.s.len - sg.s.nq + (col0 + cj) / p.G + 1 : sg.s.len;
+                for (int w = 0; w < W; w += 2) {
+                    term[i][w / 2] = pack_bf16(sum[w], sum[w + 1]);
+                    sum[w] -= bf_lo(term[i][w / 2]);
+                    sum[w + 1] -= bf_hi(term[i][w / 2]);
+                }
+            uint32_t b0, b1 = 0u;
+            if constexpr (W == 4) {
+                b0 = (tq & 1) ? (tq < 2 ? term[0][1] : term[1][1]) : (tq < 2 ? term[0][0] : term[1][0]);
+                b1 = tq == 0 ? term[2][0] : tq == 1 ? term[2][1] : 0u;
+            } else {
+                b0 = tq == 0 ? term[0][0] : tq == 1 ? term[1][0] : tq == 2 ? term[2][0] : 0u;
             }
+            q_words[(nt * 3 + 0) * 32 + lane] = b0;
+            q_words[(nt * 3 + 1) * 32 + lane] = b1;
+            q_words[(nt * 3 + 2) * 32 + lane] =         // 2^20 / up, and the softmax scale
+                __float_as_uint(p.scale_log2 * __uint_as_float((uint32_t)min(max(e + 137, 1), 254) << 23));
+        }
+        __syncthreads();
+        uint32_t qbias[NT][2];
+        float factor[NT][2];
+        int limit[NT][2];                             // end of the tokens of this segment that columns 2tq, 2tq + 1 see
+        int n_full, end_tok;                          // this warp's records that every column sees whole; end of the tokens that are here
+        {
+            const int len = state->sg.s.len, r1 = state->sg.r1, col0 = state->sg.chunk * NC;
+            const int before = len - state->sg.s.nq + 1;   // query token i sees before + i tokens
+            const int cols = min(state->sg.s.nq * p.G - col0, NC);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    qbias[nt][j] = q_words[(nt * 3 + j) * 32 + lane];
+                    factor[nt][j] = __uint_as_float(q_words[(nt * 3 + 2) * 32 + (2 * tq + j) * 4]);
+                    const int cj = nt * 8 + 2 * tq + j;
+                    limit[nt][j] = min(cj < cols ? before + (col0 + cj) / p.G : len, r1 * 16);
+                }
+            const int all = max(0, min(before + col0 / p.G, r1 * 16));
+            n_full = min(n_rec, max(0, (all / 16 - r_first + NW - 1) / NW));
+            end_tok = min(len, rec_end * 16);
         }
 
         // o[nt][2w + m][j], [j + 2]: channels 32w + 4g + 2m, + 1 of column 8nt + 2tq + j
-        float o[NT][2 * W][4], psum[NT][W][4], mrun[NT][2], lrun[NT][2];
+        float o[NT][2 * W][4], ref[NT][2], lrun[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2 * W; ++c) o[nt][c][0] = o[nt][c][1] = o[nt][c][2] = o[nt][c][3] = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) psum[nt][w][0] = psum[nt][w][1] = psum[nt][w][2] = psum[nt][w][3] = 0.f;
-            mrun[nt][0] = mrun[nt][1] = -INFINITY;
+            ref[nt][0] = ref[nt][1] = NOTHING;
             lrun[nt][0] = lrun[nt][1] = 0.f;
         }
+        uint32_t vref = 0;                             // bf16 bits, twice: no value scale of this warp so far is larger
+        float room = WEIGHT_MAX + 60.f;                // largest s - ref that keeps a weight below 2^WEIGHT_MAX: that less log2 vref
 
-        const int n_mine = n_rec;
         const int tok_a = 4 * (g >> 1) + (g & 1);      // rows g and g + 8 of the score tile are tokens tok_a and tok_a + 2
-        for (int k = 0; k < n_mine; ++k) {
+        int out_off = 0;                               // ring offset of the record that is worked on
+        auto record = [&](int k, auto masked_constant) {
+            constexpr bool MASKED = decltype(masked_constant)::value;
             cp_async_wait<STAGES - 2>();
             __syncwarp();                              // record k is here, and every lane is done with record k - 1
-            issue(sg, k + STAGES - 1);
-            const uint32_t rec = ring + (k % STAGES) * REC;
-            const int tok0 = (sg.r0 + warp + k * NW) * 16;
+            issue(k + STAGES - 1);
+            const uint32_t rec = ring + out_off;
+            out_off = out_off == (STAGES - 1) * REC ? 0 : out_off + REC;
+            const int t0 = (r_first + k * NW) * 16 + tok_a;   // this lane's tokens: t0, t0 + 2
+            auto hidden = [&](int j, int nt) { return t0 + (j & 2) >= limit[nt][j & 1]; };
 
             // scores: rows g, g + 8 = places g, g + 8 of the record
-            uint32_t ka[W], kb[W], sa[W], sb[W];       // sa, sb: W key scales, then W value scales, two a word
-            lds<D / 8>(rec + g * (D / 2) + tq * (D / 8), ka);
-            lds<D / 8>(rec + (g + 8) * (D / 2) + tq * (D / 8), kb);
-            lds<D / 8>(rec + 16 * D + g * (D / 8), sa);
-            lds<D / 8>(rec + 16 * D + (g + 8) * (D / 8), sb);
             float s[NT][4];
+            uint32_t va_scale[W / 2], vb_scale[W / 2]; // value scales of the lane's two tokens
+            {
+                uint32_t ka[W], kb[W], sa[W], sb[W];   // sa, sb: W key scales, then W value scales, two a word
+                lds<D / 8>(rec + lane * (D / 8), ka);
+                lds<D / 8>(rec + 4 * D + lane * (D / 8), kb);
+                lds<D / 8>(rec + 16 * D + g * (D / 8), sa);
+                lds<D / 8>(rec + 17 * D + g * (D / 8), sb);
+                const uint32_t ba = W == 4 && (tq & 1) ? sa[1] : sa[0], bb = W == 4 && (tq & 1) ? sb[1] : sb[0];
+                const uint32_t bias[4] = {ba, bb, ba, bb};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+                for (int nt = 0; nt < NT; ++nt) mma_bf16_0(s[nt], bias, qbias[nt][0], qbias[nt][1]);
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const uint32_t a8 = ka[w] >> 8, b8 = kb[w] >> 8;
-                const uint32_t m0[4] = {ka[w] & 0x000f000fu, kb[w] & 0x000f000fu, ka[w] & 0x00f000f0u, kb[w] & 0x00f000f0u};
-                const uint32_t m1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
-                const float ska = group_scale(sa, 0, w), skb = group_scale(sb, 0, w);
+                for (int w = 0; w < W; ++w) {
+                    const uint32_t a8 = ka[w] >> 8, b8 = kb[w] >> 8;
+                    const uint32_t m0[4] = {ka[w] & 0x000f000fu, kb[w] & 0x000f000fu, ka[w] & 0x00f000f0u, kb[w] & 0x00f000f0u};
+                    const uint32_t m1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
+                    const float ska = group_scale(sa, 0, w), skb = group_scale(sb, 0, w);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float acc[4];
-                    mma_f16_c(acc, m0, qb[nt][w][0], qb[nt][w][1], init[nt][w][0], init[nt][w][1]);
-                    mma_f16(acc, m1, qb[nt][w][2], qb[nt][w][3]);
-                    s[nt][0] = fmaf(acc[0], ska, s[nt][0]);
-                    s[nt][1] = fmaf(acc[1], ska, s[nt][1]);
-                    s[nt][2] = fmaf(acc[2], skb, s[nt][2]);
-                    s[nt][3] = fmaf(acc[3], skb, s[nt][3]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t qb[4];
+                        lds<16>(q_ops + ((nt * W + w) * 32 + lane) * 16, qb);
+                        float acc[4];
+                        mma_f16_0(acc, m0, qb[0], qb[1]);
+                        mma_f16(acc, m1, qb[2], qb[3]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[nt][j] = fmaf(acc[j], j < 2 ? ska : skb, s[nt][j]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) { va_scale[i] = sa[W / 2 + i]; vb_scale[i] = sb[W / 2 + i]; }
+            }
+            if (MASKED) {                              // scales behind the end may hold anything
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) {
+                    if (t0 >= end_tok) va_scale[i] = 0u;
+                    if (t0 + 2 >= end_tok) vb_scale[i] = 0u;
                 }
             }
-            const bool masked = tok0 + 16 > limit_min;
-            const int ta = tok0 + tok_a, tb = ta + 2;
-            const float ea = scale_bound<D>(sa), eb = scale_bound<D>(sb);
-            float mnew[NT][2];
-            bool grow = false;
+            // Weights are exp2(s - ref) * vs, ref any number that keeps them in fp16's range: it moves only when a score or a
+            // value scale leaves the room there is, which is seldom after the first record.
+            uint32_t vtop = vref;
+            float t[NT][4], top = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int i = 0; i < W / 2; ++i) vtop = __vmaxu2(vtop, __vmaxu2(va_scale[i], vb_scale[i]));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[nt][j] *= factor[nt][j & 1];
-                if (masked) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if ((j < 2 ? ta : tb) >= limit[nt][j & 1]) s[nt][j] = -INFINITY;
+                for (int j = 0; j < 4; ++j) {
+                    t[nt][j] = fmaf(s[nt][j], factor[nt][j & 1], -ref[nt][j & 1]);
+                    if (MASKED && hidden(j, nt)) t[nt][j] = -INFINITY;
+                    top = fmaxf(top, t[nt][j]);
                 }
+            if (__any_sync(0xffffffffu, top > room || vtop != vref)) {
+                // bound of every value scale so far: its exponent's largest number; the exponent is clamped to what keeps
+                // sums of weights in fp32's range (beyond it weights lose bits, far below 2^-60)
+                uint32_t v = vref & 0xffffu;           // (a scale that is NaN is for those who see it, not for the bound)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {          // maximum over the 16 tokens: two rows of this lane, then the lanes g
-                    float mx = fmaxf(s[nt][j] + ea, s[nt][j + 2] + eb);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    mnew[nt][j] = fmaxf(mrun[nt][j], mx);
-                    grow |= mnew[nt][j] > mrun[nt][j];
-                }
-            }
-            if (__any_sync(0xffffffffu, grow)) {
+                for (int i = 0; i < W / 2; ++i)
+#pragma unroll
+                    for (uint32_t x : {va_scale[i] & 0xffffu, va_scale[i] >> 16, vb_scale[i] & 0xffffu, vb_scale[i] >> 16})
+                        if (x < 0x7f80u) v = max(v, x | 0x7fu);
+                v = __reduce_max_sync(0xffffffffu, v);
+                vref = v | (v << 16);
+                const float e = fminf(fmaxf((float)((int)(v >> 7 & 0xffu) - 126), -60.f), 100.f);
+                room = WEIGHT_MAX - e;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        // (a column that has seen nothing yet: exp2(-inf) = 0 times zeros)
-                        const float c = fast_exp2(mrun[nt][j] - (mnew[nt][j] == -INFINITY ? 0.f : mnew[nt][j]));
-                        lrun[nt][j] *= c;
+                        // the column's largest score (from the score itself: t has lost it against NOTHING)
+                        float sx = -INFINITY, tx = fmaxf(t[nt][j], t[nt][j + 2]);
 #pragma unroll
-                        for (int i = 0; i < 2 * W; ++i) { o[nt][i][j] *= c; o[nt][i][j + 2] *= c; }
+                        for (int i = j; i < 4; i += 2)
+                            if (!MASKED || !hidden(i, nt)) sx = fmaxf(sx, s[nt][i] * factor[nt][j]);
 #pragma unroll
-                        for (int w = 0; w < W; ++w) { psum[nt][w][j] *= c; psum[nt][w][j + 2] *= c; }
-                        mrun[nt][j] = mnew[nt][j];
+                        for (int x = 4; x < 32; x *= 2) {
+                            sx = fmaxf(sx, __shfl_xor_sync(0xffffffffu, sx, x));
+                            tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
+                        }
+                        if (tx > room) {               // (the same for all lanes of a column)
+                            const float moved = sx + e - WEIGHT_AIM;
+                            const float c = fast_exp2(ref[nt][j] - moved);
+                            ref[nt][j] = moved;
+                            lrun[nt][j] *= c;
+#pragma unroll
+                            for (int i = 0; i < 2 * W; ++i) { o[nt][i][j] *= c; o[nt][i][j + 2] *= c; }
+#pragma unroll
+                            for (int i = j; i < 4; i += 2) {
+                                t[nt][i] = fmaf(s[nt][i], factor[nt][j], -moved);
+                                if (MASKED && hidden(i, nt)) t[nt][i] = -INFINITY;
+                            }
+                        }
                     }
             }
-            float pr[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float m = mrun[nt][j & 1] == -INFINITY ? 0.f : mrun[nt][j & 1];
-                    pr[nt][j] = fast_exp2(s[nt][j] - m);
-                }
-                lrun[nt][0] += pr[nt][0] + pr[nt][2];
-                lrun[nt][1] += pr[nt][1] + pr[nt][3];
+                for (int j = 0; j < 4; ++j) t[nt][j] = fast_exp2(t[nt][j]);
+                lrun[nt][0] += t[nt][0] + t[nt][2];
+                lrun[nt][1] += t[nt][1] + t[nt][3];
             }
 
-            // values: plane j holds tokens 4tq + 2j and + 1 of the lane's channels, matching P's rows after the move
+            // values: plane j holds tokens 4tq + 2j and + 1 of the lane's channels, matching the weights' rows after their move.
+            // Rows g take a whole byte, even channel + 16 odd channel, rows g + 8 the odd channel in its place: one logic operation
+            // less than two nibbles cost, and the difference of the rows is the even channel.  The 8 of the codes is taken out here,
+            // exactly (a packed addition of whole multiples of 2^-24; measured 10 % faster than taking it out of O by products).
             uint32_t va[W], vb[W];
             lds<D / 8>(rec + 8 * D + lane * (D / 8), va);
             lds<D / 8>(rec + 12 * D + lane * (D / 8), vb);
@@ -496,49 +635,54 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_deco
                 const uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
                 const uint32_t x = __byte_perm(va[w >> 1], va[W / 2 + (w >> 1)], sel);
                 const uint32_t y = __byte_perm(vb[w >> 1], vb[W / 2 + (w >> 1)], sel);
-                const uint32_t x8 = x >> 8, y8 = y >> 8;
-                const uint32_t m0[4] = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
-                const uint32_t m1[4] = {x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u};
-                const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                const float sva = group_scale(sa, W / 2, w) * 16384.f, svb = group_scale(sb, W / 2, w) * 16384.f;
+                const uint32_t x8 = __byte_perm(x, 0u, 0x4341u), y8 = __byte_perm(y, 0u, 0x4341u);
+                const uint32_t m0[4] = {add_f16x2(x & 0x00ff00ffu, MINUS_136), add_f16x2(x & 0x00f000f0u, MINUS_128),
+                                        add_f16x2(y & 0x00ff00ffu, MINUS_136), add_f16x2(y & 0x00f000f0u, MINUS_128)};
+                const uint32_t m1[4] = {add_f16x2(x8, MINUS_136), add_f16x2(x8 & 0x00f000f0u, MINUS_128),
+                                        add_f16x2(y8, MINUS_136), add_f16x2(y8 & 0x00f000f0u, MINUS_128)};
+                const float sva = group_scale(va_scale, 0, w), svb = group_scale(vb_scale, 0, w);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float z[4] = {pr[nt][0] * sva, pr[nt][1] * sva, pr[nt][2] * svb, pr[nt][3] * svb};
-                    if (masked) {                      // a masked token's scale may be anything, NaN included
+                    float z[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if ((j < 2 ? ta : tb) >= limit[nt][j & 1]) z[j] = 0.f;
+                    for (int j = 0; j < 4; ++j) {
+                        z[j] = t[nt][j] * (j < 2 ? sva : svb);
+                        if (MASKED && hidden(j, nt)) z[j] = 0.f;   // a live token's NaN is not for columns that do not see it
                     }
                     const uint32_t b0 = movmatrix_trans(pack_half2(z[0], z[1]));
                     const uint32_t b1 = movmatrix_trans(pack_half2(z[2], z[3]));
                     mma_f16(o[nt][2 * w], m0, b0, b1);
                     mma_f16(o[nt][2 * w + 1], m1, b0, b1);
-                    mma_f16(psum[nt][w], ones, b0, b1);
                 }
             }
-        }
+        };
+        // Records that every column sees whole, then those at the end, where columns differ.
+        const int n_mine = n_rec;
+        int k = 0;
+        for (; k < n_full; ++k) record(k, Constant<false>{});
+        for (; k < n_mine; ++k) record(k, Constant<true>{});
         cp_async_wait<0>();
         __syncwarp();
 
         // ---- the next segment's first records are on their way while this one is written
-        const Segment done = sg;
-        at += sg.r1 - sg.r0;
+        const Segment done = state->sg;
+        Segment next = done;
+        long long at = state->at;
+        const long long end = state->end, run = state->run;
         bool more = at < end;
         if (more) {
-            sg.r0 = 0;
-            if (++sg.chunk >= sg.s.chunks) {
-                sg.chunk = 0;
+            if (++next.chunk >= next.s.chunks) {
+                next.chunk = 0;
                 do {
-                    if (++sg.b == p.B) { sg.b = 0; ++sg.h; }
-                    sg.s = sequence<NC>(p, sg.b);
-                } while (sg.s.chunks == 0 && sg.h < p.Hkv);
-                more = sg.h < p.Hkv;                   // (`at` < end, so it is, while the lengths stay as they are)
+                    if (++next.b == p.B) { next.b = 0; ++next.h; }
+                    next.s = sequence<NC>(p, next.b);
+                } while (next.s.chunks == 0 && next.h < p.Hkv);
+                more = next.h < p.Hkv;                 // (`at` < end, so it is, while the lengths stay as they are)
             }
+            more = more && take(next, at, 0, end, run);   // (a run's last item may have no record in it)
         }
-        if (more) {
-            finish_segment();
-            begin(sg);
-        }
+        if (more) begin(next, query + (~item & 1) * S::QUERY);
+        const int col0 = done.chunk * NC, cols = min(done.s.nq * p.G - col0, NC);
 
         // ---- merge the warps, a tile of 8 columns at a time
         const long long slot = 2ll * blockIdx.x + (done.r0 == 0 ? 1 : 0);
@@ -551,16 +695,15 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_deco
                 l += __shfl_xor_sync(0xffffffffu, l, 4);
                 l += __shfl_xor_sync(0xffffffffu, l, 8);
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
-                if (g == 0) merge_ml[warp * 8 + c] = make_float2(mrun[nt][j], l);
+                if (g == 0) merge_ml[warp * 8 + c] = make_float2(ref[nt][j], l);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    // rows g hold sum p u 2^-24, rows g + 8 sum p u 2^-20; u = code + 8; p carries 2^14
-                    const float b0 = 8.f * psum[nt][w][j], b1 = 8.f * psum[nt][w][j + 2];
+                    // rows g hold (even + 16 odd) 2^-24, rows g + 8 odd 2^-20
                     float4 v;
-                    v.x = (o[nt][2 * w][j] * 16777216.f - b0) * 6.103515625e-05f;
-                    v.y = (o[nt][2 * w][j + 2] * 1048576.f - b1) * 6.103515625e-05f;
-                    v.z = (o[nt][2 * w + 1][j] * 16777216.f - b0) * 6.103515625e-05f;
-                    v.w = (o[nt][2 * w + 1][j + 2] * 1048576.f - b1) * 6.103515625e-05f;
+                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * 16777216.f;
+                    v.y = o[nt][2 * w][j + 2] * 1048576.f;
+                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * 16777216.f;
+                    v.w = o[nt][2 * w + 1][j + 2] * 1048576.f;
                     *reinterpret_cast<float4*>(merge + (warp * 8 + c) * S::ROW + 32 * w + 4 * g) = v;
                 }
             }
@@ -575,12 +718,11 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_deco
                     ml[w] = merge_ml[w * 8 + c];
                     M = fmaxf(M, ml[w].x);
                 }
-                const float ref = M == -INFINITY ? 0.f : M;
                 float L = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    const float wt = fast_exp2(ml[w].x - ref);
+                    const float wt = fast_exp2(ml[w].x - M);
                     const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + c) * S::ROW + d);
                     L = fmaf(ml[w].y, wt, L);
                     acc.x = fmaf(v.x, wt, acc.x); acc.y = fmaf(v.y, wt, acc.y);
@@ -605,16 +747,17 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, NT>::CTAS_PER_SM)) gqa_deco
             if (threadIdx.x == 0) {
                 const int last = atomicAdd(&p.tickets[done.c_first], 1) == n - 1;
                 if (last) p.tickets[done.c_first] = 0;  // ready for the next launch on this workspace
-                *flag = last;
+                state->last = last;
             }
             __syncthreads();
-            if (*flag) {
+            if (state->last) {
                 __threadfence();
-                combine<D, NC>(p, done, n, cols, col0, merge);
+                combine<D, NC, THREADS>(p, done, n, cols, col0, merge);
             }
             __syncthreads();
         }
         if (!more) break;
+        if (threadIdx.x == 0) { state->sg = next; state->at = at; }   // (read behind the barrier that the operands need)
     }
     report_bad_page(bad_page, p.status);
 }
@@ -630,9 +773,9 @@ static int launch(const Params& p, void* workspace, int device, cudaStream_t str
     }
     // no more CTAs than the longest possible work gives MIN_UNITS records each
     const long long chunks = ((long long)p.T * p.G + NC - 1) / NC + (p.cu_q ? p.B : 0);
-    const long long units = p.Hkv * (p.cu_q ? chunks : (long long)p.B * ((p.G + NC - 1) / NC)) * (((long long)p.N + 15) / 16);
+    const long long units = p.Hkv * (p.cu_q ? chunks : (long long)p.B * ((p.G + NC - 1) / NC)) * (SETUP + ((long long)p.N + 15) / 16);
     long long grid = (long long)sm_count(device) * S::CTAS_PER_SM;
-    if (grid > MAX_GRID / (NT == 1 ? 1 : 2)) grid = MAX_GRID / (NT == 1 ? 1 : 2);
+    if (grid > S::MAX_N) grid = S::MAX_N;
     if (grid > (units + MIN_UNITS - 1) / MIN_UNITS) grid = (units + MIN_UNITS - 1) / MIN_UNITS;
     Params q = p;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -640,7 +783,7 @@ static int launch(const Params& p, void* workspace, int device, cudaStream_t str
     q.tickets = reinterpret_cast<int*>(ws + TICKET_OFF);
     q.partial_ml = reinterpret_cast<float*>(ws + PARTIAL_OFF);
     q.partial_o = q.partial_ml + 2ll * MAX_GRID * 8 * 2;        // (NT = 2 has half the CTAs and twice the columns)
-    SKV_CUDA_TRY(launch_pdl(gqa_decode_kv4_kernel<D, NT>, dim3((unsigned)grid), dim3(THREADS), S::SMEM, stream, q));
+    SKV_CUDA_TRY(launch_pdl(gqa_decode_kv4_kernel<D, NT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, stream, q));
     SKV_CUDA_TRY(cudaGetLastError());
     return SKV_OK;
 }
@@ -674,6 +817,8 @@ int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(pool) |
          (unsigned long long)pool_stride_page | (unsigned long long)pool_stride_head) & 15)
         return fail(SKV_ERR_BAD_ARG, "q, out, the pool and its strides must be multiples of 16 bytes");
+    if (pool_stride_page < 0 || pool_stride_page > 0xffffffffll)
+        return fail(SKV_ERR_UNSUPPORTED, "a page stride of %lld bytes is not supported", pool_stride_page);
     if ((long long)T * (Hq / Hkv) > 0x7fffffffll - 16) return fail(SKV_ERR_UNSUPPORTED, "too many query rows");
     if (!workspace || workspace_bytes < kv4::workspace_bytes(D))
         return fail(SKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, kv4::workspace_bytes(D));
@@ -682,7 +827,7 @@ int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int
     if (!guard.ok) return fail(SKV_ERR_CUDA, "cannot switch to device %d", device);
     kv4::Params p = {};
     p.q = q; p.out = out; p.pool = static_cast<const uint8_t*>(pool);
-    p.sp = pool_stride_page; p.sh = pool_stride_head;
+    p.sp = (uint32_t)pool_stride_page; p.sh = pool_stride_head;
     p.page_table = page_table; p.seq_lens = seq_lens; p.cu_q = cu_q;
     p.B = B; p.T = T; p.N = N; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
     p.max_pages = max_pages; p.num_pages = num_pages; p.q_bf16 = q_is_bf16; p.out_bf16 = out_is_bf16;
