@@ -215,7 +215,7 @@ int skv_rope_quant_append(const void* qkv, int qkv_is_bf16, void* q_out, void* k
  * behind rotary_dim are not touched), not overlap it otherwise.  Hq or Hk may be 0 with null pointers.  rotary_dim even. */
 int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* positions,
                int positions_are_64, const unsigned long long* freqs, int T, int Hq, int Hk, int D,
-               int rotary_dim, int interleaved, float rope_factor, int adjoint,
+               int rotary_dim, int interleaved, double rope_factor, int adjoint,
                long long q_stride_t, long long q_stride_h, long long k_stride_t, long long k_stride_h,
                long long q_out_stride_t, long long q_out_stride_h, long long k_out_stride_t,
                long long k_out_stride_h, int device, void* stream);
@@ -237,7 +237,7 @@ int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype
  *   skv_rope_quant_append (D = 128, rows 16-byte aligned); SKV_KV_INT4: k_pool = base of the records, strides of page and
  *   head in bytes, the other pool arguments unused (D = 64 or 128, page_size 16). */
 int skv_append_tokens(const void* qkv, int qkv_is_bf16, long long qkv_stride, void* q_out, int q_out_is_bf16,
-                      const unsigned long long* rope_freqs, int rotary_dim, int interleaved, float rope_factor,
+                      const unsigned long long* rope_freqs, int rotary_dim, int interleaved, double rope_factor,
                       const void* positions, int positions_are_64, const int* cu_new, const int* page_table,
                       const int* seq_lens, void* k_pool, void* v_pool, float* k_scale_pool, float* v_scale_pool, int T, int B,
                       int Hq, int Hkv, int D, int kv_dtype, int page_size, int max_pages, int num_pages,

@@ -18,7 +18,7 @@ KV_F16, KV_I8, KV_E4M3, KV_INT4 = 0, 1, 2, 3
 QUANT_NONE, QUANT_INT8, QUANT_E4M3, QUANT_CAST = 0, 1, 2, 3
 ORDER_POSITION, ORDER_SCORE = 0, 1
 
-_vp, _i, _ll, _f, _sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t
+_vp, _i, _ll, _f, _d, _sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_double, C.c_size_t
 
 # name -> (restype, argtypes); mirrors include/skv_b200.h one to one.
 SIGNATURES = {
@@ -69,9 +69,9 @@ SIGNATURES = {
     "skv_silu_mul": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "skv_rope_quant_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
                                    _ll, _ll, _ll, _ll, _ll, _f, _vp, _i, _i, _i, _vp, _i, _vp]),
-    "skv_rotary": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i,
+    "skv_rotary": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _d, _i,
                         _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _i, _vp]),
-    "skv_append_tokens": (_i, [_vp, _i, _ll, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+    "skv_append_tokens": (_i, [_vp, _i, _ll, _vp, _i, _vp, _i, _i, _d, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                _i, _i, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _vp, _i, _vp]),
     "skv_read_tokens": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                              _ll, _ll, _ll, _ll, _ll, _vp, _i, _vp]),

@@ -10,8 +10,8 @@
 // values; all addressed through strides.
 //
 // Bound: HBM for prompts (D = 128, 16-bit activations: 256 bytes read per row, 256 written per query row, 72 per 4-bit
-// row), latency for a step.  LPR = D/8 lanes hold one row, eight channels (16 bytes) a lane; a lane keeps its token and
-// walks over heads, so its sines and cosines are computed once; U rows are loaded before the first is used.  The group
+// row), latency for a step.  LPR = D/8 lanes hold one row, eight channels (16 bytes) a lane; a block keeps a few tokens and
+// walks over heads, so sines and cosines are worked out once; U rows are worked on while the next U are on their way.  The group
 // maxima are shuffles among the lanes that share a scale; a row's partner channels (half layout) come by shuffle too.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -44,7 +44,7 @@ struct AppendParams {
     Pools c;
     long long qkv_stride;
     int T, B, Hq, Hkv, R, interleaved, pos64, q_bf16, head_splits, heads_per_split;
-    float factor;
+    double factor;
 };
 
 struct ReadParams {
@@ -76,9 +76,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, long long t, in
 }
 
 // x / s as correctly rounded division gives it, with r = 1 / s correctly rounded: one residual correction (Markstein's
-// theorem), which holds while nothing in it under- or overflows; `safe` says that s is far from both ends.
-__device__ __forceinline__ float div_by(float x, float s, float r, bool safe) {
-    if (!safe) return __fdiv_rn(x, s);
+// theorem), which holds while nothing in it under- or overflows, that is for s far from both ends of the range.
+__device__ __forceinline__ float div_by(float x, float s, float r) {
     const float q = x * r;
     return fmaf(fmaf(-q, s, x), r, q);
 }
@@ -121,14 +120,20 @@ __device__ __forceinline__ uint32_t abs_max_bits(const float (&x)[8], unsigned g
     return m;
 }
 
-__device__ __forceinline__ uint32_t nibbles8(const float (&x)[8], float s, float r, bool safe, bool zero) {
+// Codes of eight quotients.  A quotient is at most its top code and a thousandth, which rounds to the top code: no clamp.  The
+// rounding to whole numbers, ties to even, is the addition of 1.5 * 2^23 (+ 8, even too): the sum's low bits are the code
+// (+ 8), and the eight words weighted by powers of 16, less the same sum of their constant parts, are the packed nibbles --
+// half the instructions that conversions, clamps and shifts take.
+__device__ __forceinline__ uint32_t nibbles8(const float (&x)[8], float s, float r) {
     uint32_t w = 0;
+    if (div_safe(s)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = zero ? 0 : max(-7, min(7, __float2int_rn(div_by(x[i], s, r, safe))));
-        w |= (uint32_t)(c + 8) << (4 * i);
+        for (int i = 7; i >= 0; --i) w = w * 16u + __float_as_uint(__fadd_rn(div_by(x[i], s, r), 12582920.f));
+    } else {
+#pragma unroll
+        for (int i = 7; i >= 0; --i) w = w * 16u + __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), 12582920.f));
     }
-    return w;
+    return w - 0x3f400000u;                           // 0x4b400000 * 0x11111111
 }
 
 template <int D, bool IS_V>
@@ -138,8 +143,8 @@ __device__ __forceinline__ void store_kv4(const float (&x)[8], uint8_t* rec, int
     const bool finite = m < 0x7f800000u;
     const uint16_t sb = finite ? __bfloat16_as_ushort(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.f))) : (uint16_t)0x7fc0;
     const float s = bf16_bits_to_f(sb);
-    const bool zero = !finite || s == 0.f;
-    const uint32_t word = nibbles8(x, s, __frcp_rn(s), div_safe(s), zero);
+    // (a scale of zero or NaN: all codes zero.  Scales below the normal range hold no more than that either.)
+    const uint32_t word = finite && s >= 1.1754944e-38f ? nibbles8(x, s, __frcp_rn(s)) : 0x88888888u;
     const int w = l >> 2, c = l & 3;
     if (IS_V) {
         // the lane's eight channels are value chunks g = 2c (low half) and 2c + 1; the W words of one chunk sit in the lanes
@@ -168,27 +173,36 @@ __device__ __forceinline__ void store_row(const float (&x)[8], uint8_t* row, flo
     const uint32_t m = abs_max_bits<LPR>(x, group);
     const bool finite = m < 0x7f800000u;
     const float amax = __uint_as_float(m);
-    const float s = finite ? (amax > 0.f ? __fdiv_rn(amax, BITS4 ? 7.f : E4M3 ? 448.f : 127.f) : 1.f) : __uint_as_float(0x7fc00000u);
+    // 4-bit values: amax times the number nearest 1/7, which is what torch makes of amax / 7 on the GPU (decode_step's quantiser):
+    // with 15 codes many values lie exactly between two of them, and which one they take follows the last bit of the scale
+    const float top = BITS4 ? __fmul_rn(amax, 1.f / 7.f) : __fdiv_rn(amax, E4M3 ? 448.f : 127.f);
+    const float s = finite ? (amax > 0.f ? top : 1.f) : __uint_as_float(0x7fc00000u);
     const float r = __frcp_rn(s);
-    const bool safe = div_safe(s);
+    const bool any = finite && s >= 1.1754944e-38f;  // (a scale that is NaN, or below the normal range: all codes zero)
     if (BITS4) {
-        const uint32_t word = nibbles8(x, s, r, safe, !finite || s == 0.f);
+        const uint32_t word = any ? nibbles8(x, s, r) : 0x88888888u;
         if (live) *reinterpret_cast<uint32_t*>(row + l * 4) = word;
     } else {
-        uint32_t w[2] = {0u, 0u};
+        float q[8];
+        if (div_safe(s)) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            float a = 0.f, b = 0.f;
-            if (finite && s > 0.f) { a = div_by(x[i], s, r, safe); b = div_by(x[i + 1], s, r, safe); }
-            uint32_t pair;
+            for (int i = 0; i < 8; ++i) q[i] = div_by(x[i], s, r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = any ? __fdiv_rn(x[i], s) : 0.f;
+        }
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
             if (E4M3) {
-                pair = __nv_cvt_float2_to_fp8x2(make_float2(fminf(fmaxf(a, -448.f), 448.f), fminf(fmaxf(b, -448.f), 448.f)),
-                                                __NV_SATFINITE, __NV_E4M3);
-            } else {
-                pair = ((uint32_t)max(-127, min(127, __float2int_rn(a))) & 0xffu) |
-                       (((uint32_t)max(-127, min(127, __float2int_rn(b))) & 0xffu) << 8);
+                w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+                       ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16);
+            } else {                                  // the low byte of a quotient + 1.5 * 2^23 is its whole number
+                uint32_t c[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(__fadd_rn(q[4 * i + j], 12582912.f));
+                w[i] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
             }
-            w[i >> 2] |= pair << (8 * (i & 2));
         }
         if (live) *reinterpret_cast<uint2*>(row + l * 8) = make_uint2(w[0], w[1]);
     }
@@ -208,18 +222,33 @@ __device__ __forceinline__ int page_of(const Pools& c, int b, long long pos, int
     return SKV_INDEX(page, c.num_pages);
 }
 
+// 8192 tokens, 32 + 8 + 8 heads of 128 in bf16, 4-bit cache: 42.5 us (4.2 TB/s, 0.64 of a copy; 37.9 without rotation).  Bound by
+// instructions, 160 per two rows at two thirds of the issue slots; U and registers of 2 | 64, 3 | 80, 4 | 96: 43.4, 42.5, 43.9.
 template <typename T, int D, int CACHE>
-__global__ void __launch_bounds__(THREADS) append_tokens_kernel(const AppendParams p) {
-    constexpr int LPR = D / 8, U = 4;
+__global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendParams p) {
+    constexpr int LPR = D / 8, U = 3;
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, l = lane & (LPR - 1);
-    // all lanes of a warp walk over the same heads: `split` is uniform in it, its 32 / LPR rows are consecutive tokens
-    const unsigned warp = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-    const int split = (int)(warp % (unsigned)p.head_splits);
-    const long long t = (long long)(warp / (unsigned)p.head_splits) * (32 / LPR) + lane / LPR;
+    constexpr int ROWS = 32 / LPR, WARPS = THREADS / 32;
+    __shared__ float2 table[ROWS * D / 2];            // (cos, sin) of the block's tokens: [token][pair]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (LPR - 1);
+    // a block takes ROWS tokens and a share of the heads; every warp holds all its tokens and takes every fourth head
+    const int split = (int)(blockIdx.x % (unsigned)p.head_splits);
+    const long long t = (long long)(blockIdx.x / (unsigned)p.head_splits) * ROWS + lane / LPR;
     const unsigned group = 0xffffffffu;
     const bool in = t < p.T;
+    const int heads = p.Hq + 2 * p.Hkv, h_begin = split * p.heads_per_split + warp;
+    const int h_end = min(heads, (split + 1) * p.heads_per_split);
+    const int d0 = l * 8;
+
+    // rows are asked for before anything is known of their sequence (one behind the last reads the first row and drops it)
+    const T* src = static_cast<const T*>(p.qkv) + (in ? t : 0) * p.qkv_stride + d0;
+    uint4 next[U];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = ld_stream16(src + (long long)min(h0 + u * WARPS, heads - 1) * D);
+    };
+    load(h_begin);
 
     int b = in ? (int)min(t, (long long)p.B) : p.B;
     long long pos = 0;
@@ -236,44 +265,51 @@ __global__ void __launch_bounds__(THREADS) append_tokens_kernel(const AppendPara
                                        : (long long)static_cast<const int*>(p.positions)[t];
     }
 
-    // sines and cosines of the lane's channels: 8 pairs with a partner lane (half layout), 4 pairs of its own (interleaved)
-    const int h_begin = split * p.heads_per_split, h_end = min(p.Hq + 2 * p.Hkv, h_begin + p.heads_per_split);
-    const int d0 = l * 8;
+    // the lane's channels: 8 pairs with a partner lane (half layout; the first half takes the sine negative), or 4 of its own
     const bool turned = p.freqs && d0 < p.R;
     float cs[8], sn[8];
     int partner = lane;
-    if (turned && h_begin < p.Hq + p.Hkv) {
-        if (p.interleaved) {
+    if (p.freqs) {
+        const int half = p.R / 2;
+        for (int i0 = 0; i0 < ROWS * half; i0 += THREADS) {
+            const int i = min(i0 + (int)threadIdx.x, ROWS * half - 1), r = i / half;
+            const long long at = __shfl_sync(group, pos, r * LPR);
+            table[i] = rotary_cos_sin(at, p.freqs[i - r * half], p.factor);
+        }
+        __syncthreads();
+        if (turned) {
+            const float2* f = table + (lane / LPR) * half;
+            if (p.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rotary_sincos(pos, p.freqs[l * 4 + i], sn[i], cs[i]);
-        } else {
-            const bool first = d0 < p.R / 2;
-            partner = first ? lane + p.R / 16 : lane - p.R / 16;
+                for (int i = 0; i < 4; ++i) { cs[i] = f[l * 4 + i].x; sn[i] = f[l * 4 + i].y; }
+            } else {
+                const bool first = d0 < half;
+                partner = first ? lane + p.R / 16 : lane - p.R / 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                rotary_sincos(pos, p.freqs[(first ? d0 : d0 - p.R / 2) + i], sn[i], cs[i]);
-                if (first) sn[i] = -sn[i];
+                for (int i = 0; i < 8; ++i) {
+                    const float2 x = f[(first ? d0 : d0 - half) + i];
+                    cs[i] = x.x;
+                    sn[i] = first ? -x.y : x.y;
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { sn[i] *= p.factor; cs[i] *= p.factor; }
     }
 
-    const T* src = static_cast<const T*>(p.qkv) + (mine ? t : 0) * p.qkv_stride + d0;
-    for (int h0 = h_begin; h0 < h_end; h0 += U) {
+    __half* q_row = static_cast<__half*>(p.q_out) + t * p.Hq * D + d0;
+    const bool live = mine && page >= 0;
+    const long long pg = live ? page : 0;
+    for (int h0 = h_begin; h0 < h_end; h0 += U * WARPS) {
         uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            raw[u] = ld_stream16(src + (long long)min(h0 + u, h_end - 1) * D);
-#pragma unroll
-        for (int u = 0; u < U; ++u) pin_loaded(raw[u]);
+        for (int u = 0; u < U; ++u) raw[u] = next[u];
+        if (h0 + U * WARPS < h_end) load(h0 + U * WARPS);   // the next rows are on their way while these are worked on
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = h0 + u;
+            const int h = h0 + u * WARPS;
             if (h >= h_end) break;
             float x[8];
             unpack16<T>(raw[u], x);
-            if (h < p.Hq + p.Hkv && p.freqs) {
+            if (h < p.Hq + p.Hkv) {
                 if (p.interleaved) {
                     if (turned) {
 #pragma unroll
@@ -282,7 +318,7 @@ __global__ void __launch_bounds__(THREADS) append_tokens_kernel(const AppendPara
                             rotary_turn(a, c, sn[i], cs[i], x[2 * i], x[2 * i + 1]);
                         }
                     }
-                } else {
+                } else if (p.freqs) {
                     uint4 o;
                     o.x = __shfl_sync(group, raw[u].x, partner); o.y = __shfl_sync(group, raw[u].y, partner);
                     o.z = __shfl_sync(group, raw[u].z, partner); o.w = __shfl_sync(group, raw[u].w, partner);
@@ -290,23 +326,19 @@ __global__ void __launch_bounds__(THREADS) append_tokens_kernel(const AppendPara
                         float y[8];
                         unpack16<T>(o, y);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = fmaf(y[i], sn[i], __fmul_rn(x[i], cs[i]));
+                        for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(y[i], sn[i]));
                     }
                 }
-            }
-            if (h < p.Hq) {
-                if (mine) {
-                    uint4 o;
-                    o.x = pack16(x[0], x[1], p.q_bf16); o.y = pack16(x[2], x[3], p.q_bf16);
-                    o.z = pack16(x[4], x[5], p.q_bf16); o.w = pack16(x[6], x[7], p.q_bf16);
-                    *reinterpret_cast<uint4*>(static_cast<__half*>(p.q_out) + (t * p.Hq + h) * D + d0) = o;
+                if (h < p.Hq) {
+                    if (mine)
+                        *reinterpret_cast<uint4*>(q_row + (long long)h * D) =
+                            make_uint4(pack16(x[0], x[1], p.q_bf16), pack16(x[2], x[3], p.q_bf16), pack16(x[4], x[5], p.q_bf16),
+                                       pack16(x[6], x[7], p.q_bf16));
+                    continue;
                 }
-                continue;
             }
             const bool is_v = h >= p.Hq + p.Hkv;
             const int hk = h - p.Hq - (is_v ? p.Hkv : 0);
-            const bool live = mine && page >= 0;
-            const long long pg = live ? page : 0;
             if constexpr (CACHE == CACHE_KV4) {
                 uint8_t* rec = p.c.k + pg * p.c.sp + hk * p.c.sh;
                 if (is_v) store_kv4<D, true>(x, rec, slot, l, group, live);
@@ -429,7 +461,19 @@ static int make_pools(const char* who, Pools* c, int* cache, void* k_pool, void*
     return SKV_OK;
 }
 
-// Heads are split over warps until the machine is full, as in rotary.cu.
+// A block's heads (a multiple of the four that its warps take at a time): all of them for long prompts, whose blocks are many;
+// shares of them while there are fewer than four blocks an SM.
+static long long split_blocks(long long tiles, int heads, int device, int* splits, int* per) {
+    const long long want = (long long)sm_count(device) * 4;
+    const int fours = (heads + 3) / 4;
+    long long s = (want + tiles - 1) / tiles;
+    s = s < 1 ? 1 : s > fours ? fours : s;
+    *per = 4 * (int)((fours + s - 1) / s);
+    *splits = (heads + *per - 1) / *per;
+    return tiles * *splits;
+}
+
+// Heads are split over warps until the machine is full.
 static long long split_heads(long long warps, int heads, int device, int* splits, int* per) {
     const long long want = (long long)sm_count(device) * 32;
     long long s = (want + warps - 1) / warps;
@@ -470,7 +514,7 @@ using namespace skv;
 extern "C" {
 
 int skv_append_tokens(const void* qkv, int qkv_is_bf16, long long qkv_stride, void* q_out, int q_out_is_bf16,
-                      const unsigned long long* rope_freqs, int rotary_dim, int interleaved, float rope_factor,
+                      const unsigned long long* rope_freqs, int rotary_dim, int interleaved, double rope_factor,
                       const void* positions, int positions_are_64, const int* cu_new, const int* page_table,
                       const int* seq_lens, void* k_pool, void* v_pool, float* k_scale_pool, float* v_scale_pool, int T, int B,
                       int Hq, int Hkv, int D, int kv_dtype, int page_size, int max_pages, int num_pages,
@@ -497,9 +541,8 @@ int skv_append_tokens(const void* qkv, int qkv_is_bf16, long long qkv_stride, vo
     p.qkv_stride = qkv_stride;
     p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.R = rotary_dim; p.interleaved = interleaved; p.pos64 = positions_are_64;
     p.q_bf16 = q_out_is_bf16; p.factor = rope_factor;
-    const int rows = 256 / D;   // per warp
-    const long long warps = tok::split_heads(((long long)T + rows - 1) / rows, Hq + 2 * Hkv, device, &p.head_splits, &p.heads_per_split);
-    const long long blocks = (warps + tok::THREADS / 32 - 1) / (tok::THREADS / 32);
+    const int rows = 256 / D;   // per block
+    const long long blocks = tok::split_blocks(((long long)T + rows - 1) / rows, Hq + 2 * Hkv, device, &p.head_splits, &p.heads_per_split);
     if (blocks > 0x3fffffff) return fail(SKV_ERR_UNSUPPORTED, "skv_append_tokens: too many rows for one launch");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)blocks), block(tok::THREADS);

@@ -11,10 +11,11 @@
 // Angles: f_i comes as the 64-bit fixed-point fraction F_i = round(f_i / (2 pi) * 2^64) of a turn per position, so
 // position * F_i mod 2^64 is the angle's place in its turn, exact but for the rounding of f_i itself: far positions
 // (2^20 and beyond, where a 32-bit product is off by a tenth of a radian) cost two integer multiplications and need no
-// range reduction.  The upper 32 bits go to sincospif.
+// range reduction.
 //
-// Bound: HBM, one read and one write of every row.  A thread owns VEC frequencies of one token and walks over heads, so
-// that sines and cosines are computed once for the heads of its share; U rows are loaded before the first is used.
+// Bound: HBM, one read and one write of every row.  A thread keeps one vector of one token's channels and takes it from U
+// heads, all asked for at once; its block works out the sines and cosines of its tokens once, in shared memory, while the
+// rows are on their way, and every thread takes those of its channels to registers.
 #include <cuda_bf16.h>
 
 #include "skv_common.cuh"
@@ -23,132 +24,224 @@
 namespace skv {
 namespace rot {
 
-constexpr int THREADS = 128;
+constexpr int MAX_THREADS = 256;
 
 struct Params {
-    const void* src[2];         // q, k (k may be null with heads[1] == 0)
+    const void* src[2];         // q, k (k may be absent)
     void* dst[2];
     long long st[2], sh[2];     // element strides of token and head, source ...
     long long dt[2], dh[2];     // ... and destination
     const void* positions;
     const unsigned long long* freqs;   // [R / 2] turns per position, 64-bit fixed point
-    int pos64, T, Hq, H, R, tail_units, units, head_splits, heads_per_split;
-    float factor, sign;
+    int pos64, T, Hq, H, D, R;
+    int turn_units, units;      // vectors per row: the turned ones, and with those that are copied
+    int width;                  // vectors of a row that a block's threads hold at a time: units, where they fit
+    int tokens, lanes;          // a block's tokens, and threads that share one vector's heads; tokens * width * lanes threads
+    double factor;
+    float sign;
 };
 
-// N elements of T as one load or store of up to 16 bytes
-template <typename T, int N>
-struct alignas(N * sizeof(T)) Vec {
-    T v[N];
+// E elements of T as one access of up to 16 bytes (LOOSE: aligned to an element only)
+template <typename T, int E, bool LOOSE>
+struct alignas(LOOSE ? sizeof(T) : E * sizeof(T)) Vec {
+    T v[E];
 };
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float x, float& y) { y = x; }
-__device__ __forceinline__ void from_f(float x, __half& y) { y = __float2half_rn(x); }
-__device__ __forceinline__ void from_f(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
-
-template <typename T, int VEC, bool INTER>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(const Params p) {
-    constexpr int U = sizeof(T) * VEC >= 16 ? 4 : 2;   // rows in flight
-    pdl_wait_prior_grids();
-    pdl_launch_dependents();
-    const unsigned item = blockIdx.x * THREADS + threadIdx.x;   // (the launcher keeps the count below 2^31)
-    const int unit = (int)(item % (unsigned)p.units);
-    const unsigned rest = item / (unsigned)p.units;
-    const int split = (int)(rest % (unsigned)p.head_splits);
-    const long long t = rest / (unsigned)p.head_splits;
-    if (t >= p.T) return;
-    const int h_begin = split * p.heads_per_split, h_end = min(p.H, h_begin + p.heads_per_split);
-    const int nrot = p.units - p.tail_units;
-
-    if (unit >= nrot) {   // a vector of the channels behind the rotated part
-        const int d = p.R + (unit - nrot) * VEC;
-        for (int h = h_begin; h < h_end; ++h) {
-            const int w = h >= p.Hq;
-            const int hh = h - (w ? p.Hq : 0);
-            *reinterpret_cast<Vec<T, VEC>*>(static_cast<T*>(p.dst[w]) + t * p.dt[w] + hh * p.dh[w] + d) =
-                *reinterpret_cast<const Vec<T, VEC>*>(static_cast<const T*>(p.src[w]) + t * p.st[w] + hh * p.sh[w] + d);
-        }
-        return;
-    }
-
-    const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[t]
-                                  : (long long)static_cast<const int*>(p.positions)[t];
-    float cs[VEC], sn[VEC];
+// 16-bit channels are taken from and put into their words, two at a time
+template <typename T, int E>
+__device__ __forceinline__ void to_floats(const T (&v)[E], float (&x)[E]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        rotary_sincos(pos, p.freqs[unit * VEC + i], sn[i], cs[i]);
-        sn[i] *= p.sign * p.factor;
-        cs[i] *= p.factor;
-    }
-    const int c0 = INTER ? unit * 2 * VEC : unit * VEC;
-    const int c1 = INTER ? c0 + VEC : c0 + p.R / 2;
-    for (int h0 = h_begin; h0 < h_end; h0 += U) {
-        Vec<T, VEC> a[U], b[U];
+        for (int i = 0; i < E; ++i) x[i] = v[i];
+    } else if constexpr (E == 1) {
+        x[0] = static_cast<float>(v[0]);
+    } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = min(h0 + u, h_end - 1);   // (a row past the end is loaded twice and not stored)
-            const int w = h >= p.Hq;
-            const T* s = static_cast<const T*>(p.src[w]) + t * p.st[w] + (h - (w ? p.Hq : 0)) * p.sh[w];
-            a[u] = *reinterpret_cast<const Vec<T, VEC>*>(s + c0);
-            b[u] = *reinterpret_cast<const Vec<T, VEC>*>(s + c1);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + u;
-            if (h >= h_end) break;
-            const int w = h >= p.Hq;
-            Vec<T, VEC> x, y;
-            if (INTER) {   // a, b together hold 2 VEC neighbouring channels
-                T e[2 * VEC], r[2 * VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) { e[i] = a[u].v[i]; e[VEC + i] = b[u].v[i]; }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    float m, n;
-                    rotary_turn(to_f(e[2 * i]), to_f(e[2 * i + 1]), sn[i], cs[i], m, n);
-                    from_f(m, r[2 * i]);
-                    from_f(n, r[2 * i + 1]);
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) { x.v[i] = r[i]; y.v[i] = r[VEC + i]; }
+        for (int i = 0; i < E / 2; ++i) {
+            uint32_t w;
+            if constexpr (E == 2) w = (uint32_t)reinterpret_cast<const uint16_t*>(v)[0] | ((uint32_t)reinterpret_cast<const uint16_t*>(v)[1] << 16);
+            else w = reinterpret_cast<const uint32_t*>(v)[i];
+            if constexpr (__is_same(T, __half)) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                x[2 * i] = f.x; x[2 * i + 1] = f.y;
             } else {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    float m, n;
-                    rotary_turn(to_f(a[u].v[i]), to_f(b[u].v[i]), sn[i], cs[i], m, n);
-                    from_f(m, x.v[i]);
-                    from_f(n, y.v[i]);
-                }
+                x[2 * i] = __uint_as_float(w << 16); x[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
             }
-            T* d = static_cast<T*>(p.dst[w]) + t * p.dt[w] + (h - (w ? p.Hq : 0)) * p.dh[w];
-            *reinterpret_cast<Vec<T, VEC>*>(d + c0) = x;
-            *reinterpret_cast<Vec<T, VEC>*>(d + c1) = y;
+        }
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void from_floats(const float (&x)[E], T (&v)[E]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = x[i];
+    } else if constexpr (E == 1) {
+        if constexpr (__is_same(T, __half)) v[0] = __float2half_rn(x[0]);
+        else v[0] = __float2bfloat16_rn(x[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            uint32_t w;
+            if constexpr (__is_same(T, __half)) {
+                w = pack_half2(x[2 * i], x[2 * i + 1]);
+            } else {
+                const __nv_bfloat162 f = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w = *reinterpret_cast<const uint32_t*>(&f);
+            }
+            if constexpr (E == 2) {
+                reinterpret_cast<uint16_t*>(v)[0] = (uint16_t)w;
+                reinterpret_cast<uint16_t*>(v)[1] = (uint16_t)(w >> 16);
+            } else {
+                reinterpret_cast<uint32_t*>(v)[i] = w;
+            }
         }
     }
 }
 
-template <typename T, int VEC>
-static int launch(const Params& p, int interleaved, cudaStream_t st) {
-    const long long threads = (long long)p.T * p.units * p.head_splits;
-    const long long blocks = (threads + THREADS - 1) / THREADS;
-    if (threads > 0x7fffff00ll) return fail(SKV_ERR_UNSUPPORTED, "skv_rotary: too many rows for one launch");
-    SKV_CUDA_TRY(launch_pdl(interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>, dim3((unsigned)blocks),
-                            dim3(THREADS), 0, st, p));
+// A unit of a row: half layout, E channels of the first half and the E that belong to them; interleaved, E channels in a row
+// (E / 2 pairs); behind the turned part E channels in a row, copied.
+// 64 registers, four full blocks an SM: 28.3 us for that prompt (5.9 TB/s, 0.90 of a copy), 31.0 with 80.
+template <typename T, int E, bool INTER>
+__global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) {
+    constexpr int NP = INTER ? E / 2 : E;             // pairs of a unit
+    constexpr int U = INTER ? 8 : 4;                  // heads in flight per thread
+    constexpr bool LOOSE = INTER && E == 2;           // channels fetched one by one: no alignment, and rows of an odd length
+    using V = Vec<T, E, LOOSE>;
+    extern __shared__ float2 table[];                 // (cos, sin): [token][pair of the unit][unit]
+    pdl_wait_prior_grids();
+    pdl_launch_dependents();
+    const int t0 = blockIdx.x * p.tokens, nt = min(p.tokens, p.T - t0);
+    // this thread: vector `first`, `first + width`, ... of token tt, heads `lane`, `lane + lanes`, ...
+    const int first = threadIdx.x % p.width, rest = threadIdx.x / p.width;
+    const int lane = rest % p.lanes, tt = rest / p.lanes;
+    const bool live = tt < nt;
+    const long long t = t0 + (live ? tt : 0);
+
+    V a[U], b[U];
+    auto channel = [&](int u) { return u < p.turn_units ? u * E : p.R + (u - p.turn_units) * E; };
+    auto load = [&](int u, int h0) {
+        const int c = channel(u);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int h = min(h0 + k * p.lanes, p.H - 1), w = h >= p.Hq;   // (past the last head: that one again, not stored)
+            const T* s = static_cast<const T*>(p.src[w]) + t * p.st[w] + (h - (w ? p.Hq : 0)) * p.sh[w] + c;
+            if constexpr (LOOSE) {
+                a[k].v[0] = s[0];
+                a[k].v[1] = s[c + 1 < p.D ? 1 : 0];
+            } else {
+                a[k] = *reinterpret_cast<const V*>(s);
+            }
+            if (!INTER) b[k] = *reinterpret_cast<const V*>(u < p.turn_units ? s + p.R / 2 : s);
+        }
+    };
+    // the block's angles: what they need is asked for first, then the rows, and the sines are worked out while those come
+    const int pairs = p.turn_units * NP, angles = nt * pairs;
+    auto angle = [&](int i, long long& pos, unsigned long long& f) {
+        const int x = i / pairs;
+        pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + x] : (long long)static_cast<const int*>(p.positions)[t0 + x];
+        f = p.freqs[i - x * pairs];
+    };
+    auto write = [&](int i, long long pos, unsigned long long f) {
+        const int x = i / pairs, r = i - x * pairs;
+        float2 cs = rotary_cos_sin(pos, f, p.factor);
+        cs.y *= p.sign;
+        table[(x * NP + r % NP) * p.turn_units + r / NP] = cs;
+    };
+    {
+        long long pos = 0;
+        unsigned long long f = 0;
+        if (threadIdx.x < angles) angle(threadIdx.x, pos, f);
+        load(first, lane);
+        if (threadIdx.x < angles) write(threadIdx.x, pos, f);
+        for (int i = threadIdx.x + blockDim.x; i < angles; i += blockDim.x) {
+            angle(i, pos, f);
+            write(i, pos, f);
+        }
+    }
+    __syncthreads();
+    if (!live) return;
+    for (int u = first; u < p.units; u += p.width) {
+        const bool turned = u < p.turn_units;
+        float cs[NP], sn[NP];
+        if (turned) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const float2 f = table[(tt * NP + i) * p.turn_units + u];
+                cs[i] = f.x;
+                sn[i] = f.y;
+            }
+        }
+        const int c = channel(u);
+        for (int h0 = lane; h0 < p.H; h0 += U * p.lanes) {
+            if (u != first || h0 != lane) load(u, h0);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int h = h0 + k * p.lanes;
+                if (h >= p.H) break;
+                V lo = a[k], hi;
+                if (turned) {
+                    float x[E], y[E];
+                    to_floats(a[k].v, x);
+                    if constexpr (INTER) {
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) rotary_turn(x[2 * i], x[2 * i + 1], sn[i], cs[i], y[2 * i], y[2 * i + 1]);
+                        from_floats(y, lo.v);
+                    } else {
+                        float m[E], n[E];
+                        to_floats(b[k].v, y);
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) rotary_turn(x[i], y[i], sn[i], cs[i], m[i], n[i]);
+                        from_floats(m, lo.v);
+                        from_floats(n, hi.v);
+                    }
+                }
+                const int w = h >= p.Hq;
+                T* d = static_cast<T*>(p.dst[w]) + t * p.dt[w] + (h - (w ? p.Hq : 0)) * p.dh[w] + c;
+                if constexpr (LOOSE) {
+                    d[0] = lo.v[0];
+                    if (c + 1 < p.D) d[1] = lo.v[1];
+                } else {
+                    *reinterpret_cast<V*>(d) = lo;
+                }
+                if (!INTER && turned) *reinterpret_cast<V*>(d + p.R / 2) = hi;
+            }
+        }
+    }
+}
+
+template <typename T, int E, bool INTER>
+static int launch(Params& p, int tail, cudaStream_t st) {
+    constexpr int NP = INTER ? E / 2 : E, U = INTER ? 8 : 4;
+    p.turn_units = INTER ? p.R / E : p.R / 2 / E;
+    p.units = p.turn_units + (tail + E - 1) / E;
+    // Threads for every vector of a row, enough of them side by side that each takes at most U heads where a block can hold
+    // them, and as many tokens as fill a block to about 160 threads (a prompt of 8192 tokens, 40 heads of 128 in bf16: 31.2 us
+    // with 96 threads, 28.3 with 160, 36 with 256).
+    p.width = p.units < MAX_THREADS ? p.units : MAX_THREADS;
+    p.lanes = (p.H + U - 1) / U;
+    if (p.lanes * p.width > MAX_THREADS) p.lanes = MAX_THREADS / p.width;
+    p.tokens = 160 / (p.lanes * p.width);
+    if (p.tokens < 1) p.tokens = 1;
+    if (p.tokens > p.T) p.tokens = p.T;
+    const long long blocks = ((long long)p.T + p.tokens - 1) / p.tokens;
+    const size_t smem = (size_t)p.tokens * p.turn_units * NP * sizeof(float2);
+    if (smem > 48 * 1024) return fail(SKV_ERR_UNSUPPORTED, "skv_rotary: rotary_dim %d is not supported", p.R);
+    SKV_CUDA_TRY(launch_pdl(rotary_kernel<T, E, INTER>, dim3((unsigned)blocks), dim3(p.tokens * p.width * p.lanes), smem, st, p));
     SKV_CUDA_TRY(cudaGetLastError());
     return SKV_OK;
 }
 
 template <typename T>
-static int launch_vec(int vec, const Params& p, int interleaved, cudaStream_t st) {
-    switch (vec) {
-        case 8: if constexpr (sizeof(T) == 2) return launch<T, 8>(p, interleaved, st);
-        case 4: return launch<T, 4>(p, interleaved, st);
-        case 2: return launch<T, 2>(p, interleaved, st);
-        default: return launch<T, 1>(p, interleaved, st);
+static int launch_vec(int vec, Params& p, int tail, int interleaved, cudaStream_t st) {
+    if (interleaved) {
+        if (sizeof(T) == 2 && vec >= 8) return launch<T, sizeof(T) == 2 ? 8 : 4, true>(p, tail, st);
+        if (vec >= 4) return launch<T, 4, true>(p, tail, st);
+        return launch<T, 2, true>(p, tail, st);
     }
+    if (sizeof(T) == 2 && vec >= 8) return launch<T, sizeof(T) == 2 ? 8 : 4, false>(p, tail, st);
+    if (vec >= 4) return launch<T, 4, false>(p, tail, st);
+    if (vec >= 2) return launch<T, 2, false>(p, tail, st);
+    return launch<T, 1, false>(p, tail, st);
 }
 
 }  // namespace rot
@@ -158,7 +251,7 @@ using namespace skv;
 
 extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* positions,
                           int positions_are_64, const unsigned long long* freqs, int T, int Hq, int Hk, int D,
-                          int rotary_dim, int interleaved, float factor, int adjoint,
+                          int rotary_dim, int interleaved, double rope_factor, int adjoint,
                           long long q_stride_t, long long q_stride_h, long long k_stride_t, long long k_stride_h,
                           long long q_out_stride_t, long long q_out_stride_h, long long k_out_stride_t,
                           long long k_out_stride_h, int device, void* stream) {
@@ -177,11 +270,11 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
     p.st[0] = q_stride_t; p.sh[0] = q_stride_h; p.st[1] = k_stride_t; p.sh[1] = k_stride_h;
     p.dt[0] = q_out_stride_t; p.dh[0] = q_out_stride_h; p.dt[1] = k_out_stride_t; p.dh[1] = k_out_stride_h;
     p.positions = positions; p.pos64 = positions_are_64; p.freqs = freqs;
-    p.T = T; p.Hq = Hq; p.H = Hq + Hk; p.R = rotary_dim;
-    p.factor = factor; p.sign = adjoint ? -1.f : 1.f;
+    p.T = T; p.Hq = Hq; p.H = Hq + Hk; p.D = D; p.R = rotary_dim;
+    p.factor = rope_factor; p.sign = adjoint ? -1.f : 1.f;
 
-    // The widest vector that the row's two halves, its tail and every pointer and stride allow: 16 bytes where a layout
-    // is an ordinary one, down to single elements for odd rotary widths or views.
+    // The widest vector that the row's parts and every pointer and stride allow: 16 bytes where a layout is an ordinary one,
+    // down to single elements for odd rotary widths or views (interleaved: to pairs, fetched one by one).
     const int esz = dtype == 2 ? 4 : 2;
     int vec = 16 / esz;
     bool same = true;   // nothing behind the rotated part to copy when a row is rotated in place
@@ -194,19 +287,10 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
         while (bits % (vec * esz)) vec /= 2;
     }
     const int tail = same ? 0 : D - rotary_dim;
-    while ((rotary_dim / 2) % vec || tail % vec || (tail && rotary_dim % vec)) vec /= 2;
-    p.tail_units = tail / vec;
-    p.units = rotary_dim / 2 / vec + p.tail_units;
-    // Heads are split over threads until the machine is full (eight blocks of 128 threads an SM hold the loads that
-    // cover HBM's latency): a prompt's thread walks over many heads and pays for its sines once, a decode step gives
-    // every head a thread of its own.
-    const long long want = (long long)sm_count(device) * 1024;
-    long long splits = (want + (long long)T * p.units - 1) / ((long long)T * p.units);
-    splits = splits < 1 ? 1 : splits > p.H ? p.H : splits;
-    p.heads_per_split = (int)((p.H + splits - 1) / splits);
-    p.head_splits = (p.H + p.heads_per_split - 1) / p.heads_per_split;
+    const int part = interleaved ? rotary_dim : rotary_dim / 2;
+    while (part % vec || tail % vec) vec /= 2;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 0) return rot::launch_vec<__half>(vec, p, interleaved, st);
-    if (dtype == 1) return rot::launch_vec<__nv_bfloat16>(vec, p, interleaved, st);
-    return rot::launch_vec<float>(vec, p, interleaved, st);
+    if (dtype == 0) return rot::launch_vec<__half>(vec, p, tail, interleaved, st);
+    if (dtype == 1) return rot::launch_vec<__nv_bfloat16>(vec, p, tail, interleaved, st);
+    return rot::launch_vec<float>(vec, p, tail, interleaved, st);
 }

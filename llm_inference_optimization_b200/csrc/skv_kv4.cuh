@@ -30,16 +30,21 @@ template <int D> __device__ __forceinline__ int kv4_v_row(int t) {   // byte of 
 }
 template <int D> __device__ __forceinline__ int kv4_scales(int t) { return 16 * D + kv4_place(t) * (D / 8); }
 
-// sin and cos of position * f, f given as a 64-bit fixed-point fraction of a turn (see rotary.cu)
-__device__ __forceinline__ void rotary_sincos(long long pos, unsigned long long f, float& sn, float& cs) {
-    const unsigned long long phase = (unsigned long long)pos * f;
-    sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f, &sn, &cs);   // 2^-31: half turns in [-1, 1)
+// cos and sin of position * f times factor, f given as a 64-bit fixed-point fraction of a turn (see rotary.cu).  In 64 bits,
+// rounded once: rows quantised behind the rotation then take the same codes as rows rotated by the formula in 64-bit angles
+// (a last-bit difference moves one value in ten million over the border between two codes).  One thread of a block works a
+// pair out for all heads, so this is a hundredth of the kernels' work.
+__device__ __forceinline__ float2 rotary_cos_sin(long long pos, unsigned long long f, double factor) {
+    const long long phase = (long long)((unsigned long long)pos * f);
+    double sn, cs;
+    sincospi((double)phase * 1.0842021724855044e-19, &sn, &cs);   // 2^-63: half turns in [-1, 1)
+    return make_float2((float)(cs * factor), (float)(sn * factor));
 }
-
-// One pair turned; the order of rounding is written out, so that every kernel and vector width gives the same bits.
+// One pair turned; every product and sum is rounded by itself, in every kernel and at every vector width, as the formula
+// written in torch does it.
 __device__ __forceinline__ void rotary_turn(float x, float y, float sn, float cs, float& u, float& w) {
-    u = fmaf(-y, sn, __fmul_rn(x, cs));
-    w = fmaf(x, sn, __fmul_rn(y, cs));
+    u = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
+    w = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
 }
 
 }  // namespace skv
