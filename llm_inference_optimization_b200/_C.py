@@ -266,17 +266,22 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
     sees nothing gets zeros; rows behind ``cu_q[B]`` are not written.  Returns ``[T,Hq,D]`` in Q's dtype, or in that of
     ``out`` (fp16 or bf16).  No reference counterpart.
     """
-    _require(Q.is_cuda and Q.dtype in (torch.float16, torch.bfloat16) and Q.dim() == 3 and Q.is_contiguous(),
+    bf16 = Q.dtype is torch.bfloat16
+    _require(Q.is_cuda and (bf16 or Q.dtype is torch.float16) and Q.dim() == 3 and Q.is_contiguous(),
              "Q must be a contiguous fp16 or bf16 CUDA tensor [T,Hq,D]")
     T, Hq, D = Q.shape
     dev = Q.device
-    _require(pool.dtype == torch.uint8 and pool.dim() == 4 and pool.shape[2] == 18 and pool.shape[3] == D and pool.device == dev
-             and pool.stride(3) == 1 and pool.stride(2) == D, "pool must be uint8 [num_pages,Hkv,18,D] page records on Q's device")
+    _require(pool.dtype is torch.uint8 and pool.dim() == 4 and pool.shape[2:] == (18, D) and pool.device == dev,
+             "pool must be uint8 [num_pages,Hkv,18,D] page records on Q's device")
+    sp, sh, sr, sd = pool.stride()
+    _require(sd == 1 and sr == D, "pool must hold whole page records (its last two dimensions contiguous)")
     num_pages, Hkv = pool.shape[:2]
+    table = lens = cu = None
     if page_table is not None:
-        _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
+        _require(page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
                  and page_table.device == dev, "page_table must be a contiguous int32 [B,max_pages] tensor on Q's device")
         B, max_pages = page_table.shape
+        table = page_table.data_ptr()
     else:
         B = T if cu_q is None else cu_q.numel() - 1
         _require(B > 0 and num_pages % B == 0, "without a page table num_pages must be B * max_pages")
@@ -284,24 +289,26 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
     if cu_q is None:
         _require(T == B, "one query row per sequence, or cu_q")
     else:
-        _require(cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous() and cu_q.device == dev,
+        _require(cu_q.dtype is torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous() and cu_q.device == dev,
                  "cu_q must be a contiguous int32 [B+1] tensor on Q's device")
+        cu = cu_q.data_ptr()
     if seq_lens is not None:
-        _require(seq_lens.dtype == torch.int32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
+        _require(seq_lens.dtype is torch.int32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
                  and seq_lens.device == dev, "seq_lens must be a contiguous int32 [B] tensor on Q's device")
+        lens = seq_lens.data_ptr()
     N = int(max_seq_len) if max_seq_len is not None else max_pages * 16
     _require(0 < N <= max_pages * 16, "max_seq_len must be in (0, max_pages * 16]")
     if out is None:
-        out = torch.empty_like(Q)
+        out, out_bf16 = torch.empty_like(Q), bf16
     else:
-        _require(out.dtype in (torch.float16, torch.bfloat16) and out.shape == Q.shape and out.is_contiguous()
+        out_bf16 = out.dtype is torch.bfloat16
+        _require((out_bf16 or out.dtype is torch.float16) and out.shape == Q.shape and out.is_contiguous()
                  and out.device == dev, "out must be a contiguous fp16 or bf16 tensor of Q's shape on Q's device")
     lib = _lib.load()
-    ws = _workspace.scratch("gqa_kv4", lib.skv_gqa_decode_kv4_workspace_bytes(D), 8192, dev)
-    rc = lib.skv_gqa_decode_kv4(
-        Q.data_ptr(), Q.dtype == torch.bfloat16, pool.data_ptr(), None if page_table is None else page_table.data_ptr(),
-        None if seq_lens is None else seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), out.data_ptr(),
-        out.dtype == torch.bfloat16, ws.data_ptr(), ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages,
-        pool.stride(0), pool.stride(1), float(scale), _dev_index(Q), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "fused_gqa_kv4")
+    stream = _workspace.stream(dev.index)
+    ws = _workspace.scratch("gqa_kv4", lib.skv_gqa_decode_kv4_workspace_bytes(D), 8192, dev, stream)
+    rc = lib.skv_gqa_decode_kv4(Q.data_ptr(), bf16, pool.data_ptr(), table, lens, cu, out.data_ptr(), out_bf16, ws.data_ptr(),
+                                ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages, sp, sh, scale, dev.index, stream)
+    if rc:
+        _lib.check(rc, "fused_gqa_kv4")
     return out

@@ -25,16 +25,27 @@ def get(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
     return buf
 
 
-def scratch(kind: str, nbytes: int, head: int, device: torch.device) -> torch.Tensor:
+# The raw handle of a device's current stream, without building a Stream object around it (2 us of a 5 us launch).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream(index: int) -> int:
+    """Handle of the current stream of device ``index``."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def scratch(kind: str, nbytes: int, head: int, device: torch.device, handle: int) -> torch.Tensor:
     """Like :func:`get` for kernels of which only the first ``head`` bytes must be zero, and safe under graph capture.
 
-    A call that is being captured gets a buffer of the graph's own, whose head is cleared by a node of the graph: two
-    graphs, or a graph and eager calls, never share one, however their replays overlap."""
+    ``device`` has an index, ``handle`` is its current stream (:func:`stream`).  A call that is being captured gets a buffer
+    of the graph's own, whose head is cleared by a node of the graph: two graphs, or a graph and eager calls, never share
+    one, however their replays overlap."""
     if torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:head].zero_()
         return buf
-    return get(kind, nbytes, device)
+    buf = _cache.get((kind, device.index, handle))
+    return buf if buf is not None and buf.numel() >= nbytes else get(kind, nbytes, device)
 
 
 def all_of(kind: str, device: torch.device) -> list[torch.Tensor]:

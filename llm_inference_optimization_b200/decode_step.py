@@ -27,7 +27,7 @@ import torch
 import torch.distributed as dist
 from torch import Tensor
 
-from . import paged
+from . import paged, rotary
 from .sharding import HeadShard, shard_columns
 
 
@@ -43,6 +43,7 @@ class ModelConfig:
     rope_theta: float = 500000.0
     rms_eps: float = 1e-5
     init_std: float = 0.02
+    rope_scaling: dict | None = None   # frequency scaling of rotary.frequencies (the reference's Llama-3.1 model uses "llama3")
 
 
 def _matrix(seed: int, layer: int, name: str, shape, device, dtype, std) -> Tensor:
@@ -56,13 +57,17 @@ def rms_norm(x: Tensor, w: Tensor, eps: float) -> Tensor:
     return torch.nn.functional.rms_norm(x, (x.shape[-1],), w, eps)
 
 
-def rope(x: Tensor, pos: Tensor, theta: float) -> Tensor:
+def rope(x: Tensor, pos: Tensor, theta: float, scaling: dict | None = None) -> Tensor:
     """Plain rotary embedding (rotate-half form) of ``x [B, H, D]`` at integer positions ``pos [B]``."""
     D = x.shape[-1]
-    inv = 1.0 / (theta ** (torch.arange(0, D, 2, device=x.device, dtype=torch.float32) / D))
+    if scaling is None:
+        inv, factor = 1.0 / (theta ** (torch.arange(0, D, 2, device=x.device, dtype=torch.float32) / D)), 1.0
+    else:
+        freqs, factor = rotary.frequencies(D, theta, scaling)
+        inv = torch.tensor(freqs, device=x.device, dtype=torch.float32)
     ang = pos.float()[:, None] * inv[None, :]
-    cos = torch.cat([ang.cos(), ang.cos()], -1)[:, None, :]
-    sin = torch.cat([ang.sin(), ang.sin()], -1)[:, None, :]
+    cos = torch.cat([ang.cos(), ang.cos()], -1)[:, None, :] * factor
+    sin = torch.cat([ang.sin(), ang.sin()], -1)[:, None, :] * factor
     xf = x.float()
     rot = torch.cat([-xf[..., D // 2:], xf[..., :D // 2]], -1)
     return (xf * cos + rot * sin).to(x.dtype)
@@ -85,12 +90,24 @@ def quantize_rows_int4(x: Tensor):
     return (u[..., 0::2] | (u[..., 1::2] << 4)).contiguous(), scale
 
 
-class LayerCache:
-    """Paged cache of one layer on one rank, page size 16: fused FP8 page records, or with ``v_bits=4`` mixed-precision
-    records (FP8 keys, 4-bit values)."""
+def quantize_groups_int4(x: Tensor):
+    """4-bit codes (int8, -7..7) and bf16 scales = amax / 7 of every 32 channels of ``x [..., D]`` (4-bit page records)."""
+    g = x.float().unflatten(-1, (-1, 32))
+    scale = (g.abs().amax(-1) / 7.0).to(torch.bfloat16)
+    d = scale.float()[..., None]
+    codes = torch.where(d > 0, g / torch.where(d > 0, d, torch.ones_like(d)), torch.zeros_like(g))
+    return codes.round().clamp_(-7.0, 7.0).flatten(-2).to(torch.int8), scale
 
-    def __init__(self, num_pages: int, n_kv: int, device, v_bits: int = 8):
-        self.v_bits = v_bits
+
+class LayerCache:
+    """Paged cache of one layer on one rank, page size 16: fused FP8 page records, with ``v_bits=4`` mixed-precision
+    records (FP8 keys, 4-bit values), or with ``k_bits=4`` too records of 4-bit keys and values (``buf`` only)."""
+
+    def __init__(self, num_pages: int, n_kv: int, device, v_bits: int = 8, k_bits: int = 8):
+        self.v_bits, self.k_bits = v_bits, k_bits
+        if k_bits == 4:
+            self.buf = torch.zeros((num_pages, n_kv, paged.KV4_RECORD_ROWS, 128), dtype=torch.uint8, device=device)
+            return
         rows = paged.MIXED_RECORD_ROWS if v_bits == 4 else paged.RECORD_ROWS
         self.buf = torch.zeros((num_pages, n_kv, rows, 128), dtype=torch.uint8, device=device)
         views = paged.mixed_views if v_bits == 4 else paged.fused_views
@@ -102,6 +119,13 @@ class LayerCache:
         lens = seq_lens.long()
         page = page_table[torch.arange(B, device=k.device), lens // 16].long()
         slot = lens % 16
+        if self.k_bits == 4:
+            parts = paged.unpack_kv4(self.buf[page])       # the B pages that receive a token, taken apart and put back
+            b = torch.arange(B, device=k.device)
+            for part, new in zip(parts, (*quantize_groups_int4(k), *quantize_groups_int4(v))):
+                part[b, :, slot] = new
+            self.buf[page] = paged.pack_kv4(*parts)
+            return
         kc, ksc = quantize_rows_e4m3(k)
         vc, vsc = quantize_rows_int4(v) if self.v_bits == 4 else quantize_rows_e4m3(v)
         self.k.view(torch.uint8)[page, :, slot] = kc.view(torch.uint8)
@@ -117,6 +141,8 @@ def kernel_attention(q: Tensor, cache: LayerCache, page_table: Tensor, seq_lens:
                      max_seq_len: int) -> Tensor:
     """The product path: paged FP8 decode attention on the sm_100a kernel (fp16 query in, fp16 out)."""
     from . import _C
+    if cache.k_bits == 4:
+        return _C.fused_gqa_kv4(q.to(torch.float16).contiguous(), cache.buf, page_table, seq_lens, scale, max_seq_len=max_seq_len)
     return _C.fused_gqa_paged(q.to(torch.float16).contiguous(), cache.k, cache.v, cache.ks, cache.vs, page_table,
                               seq_lens, scale, max_seq_len=max_seq_len, v_bits=cache.v_bits)
 
@@ -126,7 +152,7 @@ class DecodeModel:
 
     def __init__(self, cfg: ModelConfig, shard: HeadShard, device, *, seed: int = 4, dtype=torch.bfloat16,
                  attention: AttentionFn = kernel_attention, group=None, layer_modes: list[str] | None = None,
-                 quest_block: int = 64, quest_top_k: int = 8, skinny_gemm: bool = False, v_bits: int = 8):
+                 quest_block: int = 64, quest_top_k: int = 8, skinny_gemm: bool = False, v_bits: int = 8, k_bits: int = 8):
         """``layer_modes``: per layer ``"dense"`` (attention over the whole cache) or ``"quest"`` (block-sparse: the
         ``quest_top_k`` blocks of ``quest_block`` tokens with the highest min/max upper-bound score per query head).
         The reference's layer sweep found sparse attention harmless in the first half of the layers only
@@ -146,11 +172,19 @@ class DecodeModel:
         if v_bits not in (4, 8):
             raise ValueError("v_bits must be 4 or 8")
         self.v_bits = v_bits
+        # 4 (with v_bits=4): keys in 4 bits too (144 bytes per token and head); such a model also takes prompts (extend)
+        if k_bits not in (4, 8) or (k_bits == 4 and v_bits != 4):
+            raise ValueError("k_bits must be 8, or 4 together with v_bits=4")
+        self.k_bits = k_bits
         self.metas: list[Tensor | None] = []
         self.set_layer_modes(layer_modes)
         # the fused RoPE + quantise + append kernel needs fp16/bf16 activations on a CUDA device
         self.fused_glue = (self.device.type == "cuda" and dtype in (torch.float16, torch.bfloat16)
                            and attention is kernel_attention)
+        # scaled frequencies and 4-bit keys go through paged.append_tokens; the one-token append kernel has neither
+        self.rope = None
+        if self.fused_glue and (k_bits == 4 or cfg.rope_scaling is not None):
+            self.rope = rotary.RotaryEmbedding(cfg.D, cfg.rope_theta, scaling=cfg.rope_scaling, device=self.device)
         self.fused_allreduce = False   # see enable_fused_allreduce
         D, hid = cfg.D, cfg.hidden
         qs = slice(shard.q_heads.start * D, shard.q_heads.stop * D)
@@ -190,6 +224,8 @@ class DecodeModel:
         modes = list(layer_modes) if layer_modes is not None else ["dense"] * self.cfg.layers
         if len(modes) != self.cfg.layers or any(m not in ("dense", "quest") for m in modes):
             raise ValueError("layer_modes must name 'dense' or 'quest' for every layer")
+        if "quest" in modes and (self.k_bits == 4 or self.cfg.rope_scaling is not None):
+            raise ValueError("block-sparse layers need 8-bit keys and unscaled rotary frequencies")
         if self.v_bits == 4 and "quest" in modes and self.quest_block * self.quest_top_k > 512:
             raise ValueError("block-sparse layers over 4-bit values gather at most 512 tokens (quest_block * quest_top_k)")
         self.layer_modes = modes
@@ -200,6 +236,8 @@ class DecodeModel:
             self._build_missing_metas()
 
     def _layer_kv(self, cache: "LayerCache", lens: Tensor):
+        if cache.k_bits == 4:
+            return paged.PagedKV4(cache.buf, self.page_table, lens, lens.numel())
         return paged.PagedKV(cache.k, cache.v, cache.ks, cache.vs, self.page_table, lens, lens.numel(), v_bits=cache.v_bits)
 
     def _build_missing_metas(self) -> None:
@@ -245,10 +283,17 @@ class DecodeModel:
         self.caches = []
         gd = torch.Generator(device=dev)
         for l in range(cfg.layers):
-            c = LayerCache(total, self.shard.n_kv, dev, self.v_bits)
+            c = LayerCache(total, self.shard.n_kv, dev, self.v_bits, self.k_bits)
             for i, head in enumerate(self.shard.kv_heads):  # keyed by the GLOBAL head: same bytes at every TP degree
                 gd.manual_seed((seed * 7919 + l * 131 + head) & 0x7FFFFFFF)
-                if fill == "normal":
+                if self.k_bits == 4 and fill in ("normal", "random_codes"):
+                    if fill == "normal":
+                        k4, v4 = (quantize_groups_int4(torch.randn((total, 1, 16, 128), generator=gd, device=dev)) for _ in range(2))
+                        c.buf[:, i:i + 1].copy_(paged.pack_kv4(*k4, *v4))
+                    else:
+                        c.buf[:, i].copy_(torch.randint(0, 256, (total, 18, 128), generator=gd, device=dev, dtype=torch.uint8))
+                        c.buf[:, i, 16:].view(torch.bfloat16).copy_(torch.rand((total, 2, 64), generator=gd, device=dev) * 0.2 + 0.3)
+                elif fill == "normal":
                     for dst, dsc, quant in ((c.k, c.ks, quantize_rows_e4m3),
                                             (c.v, c.vs, quantize_rows_int4 if self.v_bits == 4 else quantize_rows_e4m3)):
                         codes, sc = quant(torch.randn((total, 16, 128), generator=gd, device=dev))
@@ -317,17 +362,24 @@ class DecodeModel:
         return torch.matmul(x, w, out=out) if out is not None else x @ w
 
     def _fused_attention(self, li: int, qkv: Tensor, cache: "LayerCache", pos: Tensor, new_lens: Tensor, scale: float,
-                         dtype) -> Tensor:
+                         dtype, cu: Tensor | None = None) -> Tensor:
         """RoPE + quantise + append (one launch, which also keeps a sparse layer's block metadata current), then the
         layer's attention: dense over the whole paged cache, or Quest block-sparse; ``[B, n_q, D]`` in ``dtype``."""
         from . import _C
         sh, D, B = self.shard, self.cfg.D, qkv.shape[0]
         sparse = self.layer_modes[li] == "quest"
+        a = torch.empty((B, sh.n_q, D), dtype=dtype, device=qkv.device)
+        if self.rope is not None:
+            q = paged.append_tokens(qkv, self._layer_kv(cache, pos), sh.n_q, self.rope, cu_new=cu)
+            if cache.k_bits == 4:
+                return self._layer_kv(cache, new_lens).decode(q, scale, cu_q=cu, max_seq_len=self.max_seq_len, out=a)
+            _C.fused_gqa_paged(q, cache.k, cache.v, cache.ks, cache.vs, self.page_table, new_lens, scale,
+                               max_seq_len=self.max_seq_len, out=a, v_bits=cache.v_bits, after_append=self.overlap_append)
+            return a
         q = paged.rope_quant_append(qkv, self._layer_kv(cache, pos), sh.n_q, self.cfg.rope_theta,
                                     meta=self.metas[li] if sparse else None, block_size=self.quest_block)
         if sparse:
             return self._quest_attention(q, li, new_lens, scale, meta_is_current=True).to(dtype)
-        a = torch.empty((B, sh.n_q, D), dtype=dtype, device=qkv.device)
         # the append kernel above is the launch right before this one and wrote only q and position new_lens - 1
         _C.fused_gqa_paged(q, cache.k, cache.v, cache.ks, cache.vs, self.page_table, new_lens, scale,
                            max_seq_len=self.max_seq_len, out=a, v_bits=cache.v_bits, after_append=self.overlap_append)
@@ -347,6 +399,32 @@ class DecodeModel:
         self.arn = glue.AllReduceNorm(batch, self.cfg.hidden, self.dtype, self.device, self.group, protocol=protocol)
         self.fused_allreduce = True
 
+    def _fused_layers(self, x: Tensor, pos: Tensor, new_lens: Tensor, scale: float, cu: Tensor | None = None) -> Tensor:
+        """Every layer over the rows of ``x`` (updated in place); returns the normalised rows that the logits are made of."""
+        from . import glue
+        sh, eps, delta = self.shard, self.cfg.rms_eps, None
+        for li, (w, cache) in enumerate(zip(self.layers, self.caches)):
+            h = glue.residual_rmsnorm(x, delta, w["n1"], eps)
+            a = self._fused_attention(li, self._mm(h, w["wqkv"]), cache, pos, new_lens, scale, x.dtype, cu)
+            o = self._all_reduce(self._mm(a.view(x.shape[0], sh.n_q * self.cfg.D), w["wo"]))
+            h = glue.residual_rmsnorm(x, o, w["n2"], eps)
+            delta = self._all_reduce(self._mm(glue.silu_mul(self._mm(h, w["wgu"])), w["wd"]))
+        return glue.residual_rmsnorm(x, delta, self.final_norm, eps)
+
+    def extend(self, tokens: Tensor, cu_new: Tensor) -> Tensor:
+        """Take any number of new tokens per sequence: a prompt, a chunk of one, drafted tokens to be checked.
+
+        ``tokens [T]`` int64, sequence b's new ones at ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``, ``cu_new[B] == T``); each
+        attends to its sequence up to itself.  Returns logits ``[T, vocab]`` and advances ``seq_lens`` by the counts
+        (a caller that rejects drafted tokens subtracts them again).  Models with 4-bit keys and values on a GPU."""
+        if not (self.fused_glue and self.k_bits == 4):
+            raise RuntimeError("extend needs the CUDA glue path and a cache of 4-bit keys and values (k_bits=4, v_bits=4)")
+        counts = cu_new[1:] - cu_new[:-1]
+        new_lens = self.seq_lens + counts
+        h = self._fused_layers(self.embed[tokens], self.seq_lens, new_lens, 1.0 / math.sqrt(self.cfg.D), cu_new)
+        self.seq_lens.add_(counts)
+        return self._logits(h)
+
     def step(self, tokens: Tensor) -> Tensor:
         """Decode one token per sequence: ``tokens [B]`` int64 -> logits ``[B, vocab]``; advances ``seq_lens``."""
         cfg, sh = self.cfg, self.shard
@@ -360,26 +438,18 @@ class DecodeModel:
             # Per layer: residual+RMSNorm, qkv GEMM, RoPE+quantise+append, attention (writing the model dtype),
             # o_proj GEMM, residual+RMSNorm, gate/up GEMM, SiLU*up, down GEMM -- four of our launches and four GEMMs.
             # The residual stream x is updated in place; `delta` is the MLP output still to be added to it.
-            from . import _C, glue
             if self.fused_allreduce:
                 return self._step_fused_allreduce(x, pos, new_lens, scale)
-            delta = None
-            for li, (w, cache) in enumerate(zip(self.layers, self.caches)):
-                h = glue.residual_rmsnorm(x, delta, w["n1"], cfg.rms_eps)
-                qkv = self._mm(h, w["wqkv"])
-                a = self._fused_attention(li, qkv, cache, pos, new_lens, scale, x.dtype)
-                o = self._all_reduce(self._mm(a.view(B, sh.n_q * D), w["wo"]))
-                h = glue.residual_rmsnorm(x, o, w["n2"], cfg.rms_eps)
-                delta = self._all_reduce(self._mm(glue.silu_mul(self._mm(h, w["wgu"])), w["wd"]))
+            h = self._fused_layers(x, pos, new_lens, scale)
             self.seq_lens.add_(1)
-            return self._logits(glue.residual_rmsnorm(x, delta, self.final_norm, cfg.rms_eps))
+            return self._logits(h)
         for li, (w, cache) in enumerate(zip(self.layers, self.caches)):
             h = rms_norm(x, w["n1"], cfg.rms_eps)
             qkv = h @ w["wqkv"]
             q = qkv[:, :sh.n_q * D].view(B, sh.n_q, D)
             k = qkv[:, sh.n_q * D:(sh.n_q + sh.n_kv) * D].view(B, sh.n_kv, D)
             v = qkv[:, (sh.n_q + sh.n_kv) * D:].view(B, sh.n_kv, D)
-            q, k = rope(q, pos, cfg.rope_theta), rope(k, pos, cfg.rope_theta)
+            q, k = (rope(t, pos, cfg.rope_theta, cfg.rope_scaling) for t in (q, k))
             cache.append(k, v, self.page_table, pos)
             if self.layer_modes[li] == "quest":
                 a = self._quest_attention(q.to(torch.float16).contiguous(), li, new_lens, scale, meta_is_current=False)

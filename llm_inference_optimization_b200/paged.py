@@ -293,32 +293,34 @@ def unpack_kv4(buf: Tensor):
 
 
 def _token_cache(kv):
-    """Pool arguments of the append / read kernels, in their order, up to the strides; and (Hkv, D, device)."""
+    """Arguments of the append / read kernels that describe the cache -- the four pools, then format, page size, pages per
+    sequence, pages, strides -- with the page table's pointer and (Hkv, D, device)."""
     if isinstance(kv, PagedKV4):
         b = kv.buf
-        _C._require(b.is_cuda and b.dtype == torch.uint8 and b.dim() == 4 and b.shape[2] == KV4_RECORD_ROWS and b.shape[3] in (64, 128)
-                    and b.stride(3) == 1 and b.stride(2) == b.shape[3], "not a cache of 4-bit page records")
-        _, Hkv, _, D = b.shape
-        pools, fmt, strides, pages = (b.data_ptr(), None, None, None), _lib.KV_INT4, (b.stride(0), b.stride(1), 0, 0, 0), b.shape[0]
-        dev, size = b.device, 16
+        pages, Hkv, rows, D = b.shape
+        sp, sh, sr, sd = b.stride()
+        _C._require(b.is_cuda and b.dtype is torch.uint8 and rows == KV4_RECORD_ROWS and D in (64, 128) and sd == 1 and sr == D,
+                    "not a cache of 4-bit page records")
+        pools, layout, dev = (b.data_ptr(), None, None, None), (_lib.KV_INT4, 16, kv.max_pages, pages, sp, sh, 0, 0, 0), b.device
     else:
         strides = _pool_args(kv)
         pages, Hkv, size, D = kv.k_pool.shape
         pools = (kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr())
-        fmt = _C._code_dtype(kv.k_pool) | (_C.SKV_V_INT4 if kv.v_bits == 4 else 0)
+        layout = (_C._code_dtype(kv.k_pool) | (_C.SKV_V_INT4 if kv.v_bits == 4 else 0), size, kv.max_pages, pages, *strides)
         dev = kv.k_pool.device
-    t = kv.page_table
-    if t is not None:
-        _C._require(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == kv.batch and t.is_contiguous() and t.device == dev,
-                    "page_table must be a contiguous int32 [B,max_pages] tensor on the cache's device")
+    table = kv.page_table
+    if table is not None:
+        _C._require(table.dtype is torch.int32 and table.dim() == 2 and table.shape[0] == kv.batch and table.is_contiguous()
+                    and table.device == dev, "page_table must be a contiguous int32 [B,max_pages] tensor on the cache's device")
+        table = table.data_ptr()
     else:
         _C._require(pages % kv.batch == 0, "without a page table num_pages must be B * max_pages")
-    return pools, fmt, (size, kv.max_pages, pages, *strides), Hkv, D, dev
+    return pools, layout, table, Hkv, D, dev
 
 
-def _int32(t: Tensor, shape, dev, what: str) -> int:
-    _C._require(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous() and t.device == dev,
-                f"{what} must be a contiguous int32 {list(shape)} tensor on the cache's device")
+def _int32(t: Tensor, n: int, dev, what: str) -> int:
+    if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == dev):
+        raise RuntimeError(f"{what} must be a contiguous int32 [{n}] tensor on the cache's device")
     return t.data_ptr()
 
 
@@ -336,33 +338,37 @@ def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, 
     int32 device tensor of one element).  Serves ``PagedKV4`` (D 64 or 128) and every ``PagedKV`` (D 128); a rotary width
     must be a multiple of 16 (interleaved: of 8).  Block metadata is not kept current: rebuild it (``build_block_meta``).
     """
-    pools, fmt, geometry, Hkv, D, dev = _token_cache(kv)
-    _C._require(qkv.device == dev and qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.dtype in (torch.float16, torch.bfloat16)
-                and Hq >= 0 and qkv.shape[1] == (Hq + 2 * Hkv) * D,
+    pools, layout, table, Hkv, D, dev = _token_cache(kv)
+    bf16 = qkv.dtype is torch.bfloat16
+    _C._require(qkv.device == dev and qkv.dim() == 2 and (bf16 or qkv.dtype is torch.float16) and Hq >= 0
+                and qkv.shape[1] == (Hq + 2 * Hkv) * D and qkv.stride(1) == 1,
                 "qkv must be fp16/bf16 [T,(Hq+2Hkv)*D] on the cache's device, channels contiguous")
     T, B = qkv.shape[0], kv.batch
     _C._require(kv.seq_lens is not None, "the cache needs seq_lens")
-    lens = _int32(kv.seq_lens, (B,), dev, "seq_lens")
+    lens = _int32(kv.seq_lens, B, dev, "seq_lens")
     if cu_new is None:
         _C._require(T == B, "one row per sequence, or cu_new")
-    freqs, width, inter, factor = (None, 0, 0, 1.0) if rope is None else rope.kernel_args(D, dev)
-    if positions is not None:
-        _C._require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (T,) and positions.is_contiguous()
-                    and positions.device == dev, "positions must be a contiguous int32 or int64 [T] tensor on the cache's device")
-    if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=dev)
     else:
-        _C._require(q_out.dtype in (torch.float16, torch.bfloat16) and q_out.shape == (T, Hq, D) and q_out.is_contiguous()
+        cu_new = _int32(cu_new, B + 1, dev, "cu_new")
+    freqs, width, inter, factor = (None, 0, 0, 1.0) if rope is None else rope.kernel_args(D, dev)
+    pos64 = False
+    if positions is not None:
+        pos64 = positions.dtype is torch.int64
+        _C._require((pos64 or positions.dtype is torch.int32) and positions.shape == (T,) and positions.is_contiguous()
+                    and positions.device == dev, "positions must be a contiguous int32 or int64 [T] tensor on the cache's device")
+        positions = positions.data_ptr()
+    if q_out is None:
+        q_out, q_bf16 = qkv.new_empty((T, Hq, D), dtype=torch.float16), False
+    else:
+        q_bf16 = q_out.dtype is torch.bfloat16
+        _C._require((q_bf16 or q_out.dtype is torch.float16) and q_out.shape == (T, Hq, D) and q_out.is_contiguous()
                     and q_out.device == dev, "q_out must be a contiguous fp16 or bf16 [T,Hq,D] tensor on the cache's device")
     rc = _lib.load().skv_append_tokens(
-        qkv.data_ptr(), qkv.dtype == torch.bfloat16, qkv.stride(0) if T > 1 else qkv.shape[1], q_out.data_ptr(),
-        q_out.dtype == torch.bfloat16, freqs, width, inter, factor, None if positions is None else positions.data_ptr(),
-        positions is not None and positions.dtype == torch.int64,
-        None if cu_new is None else _int32(cu_new, (B + 1,), dev, "cu_new"),
-        None if kv.page_table is None else kv.page_table.data_ptr(), lens, *pools, T, B, Hq, Hkv, D, fmt, *geometry,
-        None if status is None else _int32(status, (1,), dev, "status"), _C._dev_index(qkv),
-        torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "append_tokens")
+        qkv.data_ptr(), bf16, qkv.stride(0) if T > 1 else qkv.shape[1], q_out.data_ptr(), q_bf16, freqs, width, inter, factor,
+        positions, pos64, cu_new, table, lens, *pools, T, B, Hq, Hkv, D, *layout,
+        None if status is None else _int32(status, 1, dev, "status"), dev.index, _workspace.stream(dev.index))
+    if rc:
+        _lib.check(rc, "append_tokens")
     return q_out
 
 
@@ -374,17 +380,18 @@ def read_tokens(kv: "PagedKV | PagedKV4", cu: Tensor, rows: int, *, starts: Tens
     ``None``: from 0) of sequence b: the prefix that a chunk of prompt attends to through another kernel, or a check of what
     was stored.  ``kv.seq_lens`` is not consulted.  Rows behind ``cu[B]`` are not written; a position without a page reads as
     zeros (``status`` as in :func:`append_tokens`)."""
-    pools, fmt, geometry, Hkv, D, dev = _token_cache(kv)
-    _C._require(dtype in (torch.float16, torch.bfloat16) and rows >= 0, "read_tokens returns fp16 or bf16 rows")
+    pools, layout, table, Hkv, D, dev = _token_cache(kv)
+    _C._require((dtype is torch.float16 or dtype is torch.bfloat16) and rows >= 0, "read_tokens returns fp16 or bf16 rows")
     B = kv.batch
+    cu = _int32(cu, B + 1, dev, "cu")
     K = torch.empty((rows, Hkv, D), dtype=dtype, device=dev)
     V = torch.empty_like(K)
     rc = _lib.load().skv_read_tokens(
-        *pools, None if kv.page_table is None else kv.page_table.data_ptr(), _int32(cu, (B + 1,), dev, "cu"),
-        None if starts is None else _int32(starts, (B,), dev, "starts"), K.data_ptr(), V.data_ptr(), dtype == torch.bfloat16,
-        rows, B, Hkv, D, fmt, *geometry, None if status is None else _int32(status, (1,), dev, "status"), _C._dev_index(K),
-        torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "read_tokens")
+        *pools, table, cu, None if starts is None else _int32(starts, B, dev, "starts"), K.data_ptr(), V.data_ptr(),
+        dtype is torch.bfloat16, rows, B, Hkv, D, *layout, None if status is None else _int32(status, 1, dev, "status"),
+        dev.index, _workspace.stream(dev.index))
+    if rc:
+        _lib.check(rc, "read_tokens")
     return K, V
 
 

@@ -11,7 +11,7 @@ import math
 import torch
 from torch import Tensor
 
-from . import _C, _lib
+from . import _C, _lib, _workspace
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _SCALING_KEYS = {"linear": {"factor"}, "ntk": {"factor"},
@@ -92,9 +92,10 @@ class RotaryEmbedding:
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=device)
 
     def kernel_args(self, head_dim: int, device: torch.device):
-        _C._require(self.head_dim == head_dim, f"the rotation is for head_dim {self.head_dim}, not {head_dim}")
-        _C._require(self.turns.device == device, "the rotation lives on another device")
-        return self.turns.data_ptr(), self.rotary_dim, int(self.layout == "interleaved"), self.factor
+        """What the kernels take of this object, for rows of ``head_dim`` channels on ``device``."""
+        if self.head_dim != head_dim or self.turns.device != device:
+            raise RuntimeError(f"the rotation is for head_dim {self.head_dim} on {self.turns.device}, not {head_dim} on {device}")
+        return self.turns.data_ptr(), self.rotary_dim, self.layout == "interleaved", self.factor
 
     def apply(self, positions: Tensor, q: Tensor, k: Tensor | None = None, *, adjoint: bool = False, inplace: bool = False):
         """Rotate ``q [T,Hq,D]`` (and ``k [T,Hk,D]``) at ``positions [T]`` (int32 or int64) in one launch.
@@ -103,26 +104,30 @@ class RotaryEmbedding:
         fused projection.  Returns new contiguous tensors, or the inputs with ``inplace``.  ``adjoint`` applies the
         transposed map: given gradients of the outputs it returns those of the inputs.  No autograd graph is recorded, and
         inputs that would need one are refused."""
-        _C._require(q.is_cuda and q.dim() == 3 and q.dtype in _DTYPES and q.shape[2] == self.head_dim and q.stride(2) == 1,
-                    "q must be an fp16, bf16 or fp32 CUDA tensor [T,H,head_dim] with contiguous channels")
-        dev, T = q.device, q.shape[0]
-        freqs, R, inter, factor = self.kernel_args(q.shape[2], dev)
-        _C._require(positions.dtype in (torch.int32, torch.int64) and positions.shape == (T,) and positions.is_contiguous()
+        _C._require(q.is_cuda and q.dim() == 3 and q.dtype in _DTYPES, "q must be an fp16, bf16 or fp32 CUDA tensor [T,H,head_dim]")
+        dev = q.device
+        T, Hq, D = q.shape
+        st, sh, sd = q.stride()
+        freqs, R, inter, factor = self.kernel_args(D, dev)
+        pos64 = positions.dtype is torch.int64
+        _C._require((pos64 or positions.dtype is torch.int32) and positions.shape == (T,) and positions.is_contiguous()
                     and positions.device == dev, "positions must be a contiguous int32 or int64 [T] tensor on q's device")
+        _C._require(sd == 1 or D == 1, "the channels of q must be contiguous")
         _C._require(not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))),
                     "apply records no autograd graph: call it under no_grad and use adjoint=True for the gradient")
+        qo = q if inplace else torch.empty_like(q, memory_format=torch.contiguous_format)
+        Hk, kp, kop, ko, strides = 0, None, None, None, (0, 0)
         if k is not None:
-            _C._require(k.dim() == 3 and k.dtype == q.dtype and k.shape[0] == T and k.shape[2] == q.shape[2] and k.stride(2) == 1
+            _C._require(k.dim() == 3 and k.dtype is q.dtype and k.shape[0] == T and k.shape[2] == D and k.stride(2) == 1
                         and k.device == dev, "k must be [T,Hk,head_dim] of q's dtype on q's device with contiguous channels")
-        qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ko = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
-        if q.shape[1] + (0 if k is None else k.shape[1]):
+            Hk, kp = k.shape[1], k.data_ptr()
+            ko = k if inplace else torch.empty_like(k, memory_format=torch.contiguous_format)
+            kop, strides = ko.data_ptr(), k.stride()[:2]
+        if Hq + Hk:
             rc = _lib.load().skv_rotary(
-                q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr(),
-                _DTYPES[q.dtype], positions.data_ptr(), positions.dtype == torch.int64, freqs, T, q.shape[1],
-                0 if k is None else k.shape[1], q.shape[2], R, inter, factor, adjoint, q.stride(0), q.stride(1),
-                *((0, 0) if k is None else (k.stride(0), k.stride(1))), qo.stride(0), qo.stride(1),
-                *((0, 0) if k is None else (ko.stride(0), ko.stride(1))), _C._dev_index(q),
-                torch.cuda.current_stream(dev).cuda_stream)
-            _lib.check(rc, "rotary")
+                q.data_ptr(), kp, qo.data_ptr(), kop, _DTYPES[q.dtype], positions.data_ptr(), pos64, freqs, T, Hq, Hk, D, R, inter,
+                factor, adjoint, st, sh, *strides, *((st, sh) if inplace else (Hq * D, D)), *(strides if inplace else (Hk * D, D)),
+                dev.index, _workspace.stream(dev.index))
+            if rc:
+                _lib.check(rc, "rotary")
         return qo if k is None else (qo, ko)
