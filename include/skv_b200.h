@@ -261,13 +261,14 @@ int skv_read_tokens(const void* k_pool, const void* v_pool, const float* k_scale
  * sequence b, query i of n sees positions < seq_lens[b] - n + i + 1 (none: zeros); NULL: one query per sequence, T = B.
  * Rows behind cu_q[B] of out are left alone.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
  * skv_gqa_decode_paged.  pool strides in bytes.  D = 64 or 128, any Hq / Hkv.  The result does not depend on timing.
- * Workspace: skv_gqa_decode_kv4_workspace_bytes(D), status word at offset 0; its first 8192 bytes are zero before the
- * first use and left reusable. */
+ * A page-table entry outside [0, num_pages) reads page 0 and sets SKV_DEV_BAD_PAGE in *status (optional int32 device word;
+ * NULL: the workspace's, at offset 0).  Workspace: skv_gqa_decode_kv4_workspace_bytes(D); its first 8192 bytes are zero
+ * before the first use and left reusable. */
 size_t skv_gqa_decode_kv4_workspace_bytes(int D);
 int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int* page_table, const int* seq_lens,
                        const int* cu_q, void* out, int out_is_bf16, void* workspace, size_t workspace_bytes, int T, int B, int N,
                        int Hq, int Hkv, int D, int max_pages, int num_pages, long long pool_stride_page,
-                       long long pool_stride_head, float scale, int device, void* stream);
+                       long long pool_stride_head, float scale, int* status, int device, void* stream);
 
 /* ---- token-sparse decode ----------------------------------------------------------
  * Replaces kv_evict_quant_forward(Q, K, V, top_k, use_int8=false)  (csrc/kernels/kv_evict_quant.cu:272-364,

@@ -255,7 +255,8 @@ def fused_gqa_paged(Q: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, 
 
 
 def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: Tensor | None, scale: float, *,
-                  cu_q: Tensor | None = None, max_seq_len: int | None = None, out: Tensor | None = None) -> Tensor:
+                  cu_q: Tensor | None = None, max_seq_len: int | None = None, out: Tensor | None = None,
+                  status: Tensor | None = None) -> Tensor:
     """Dense GQA attention over a paged cache whose keys and values are held in 4 bits (``skv_gqa_decode_kv4``).
 
     Q ``[T,Hq,D]`` fp16 or bf16, D 64 or 128; ``pool`` uint8 ``[num_pages,Hkv,18,D]`` page records of 16 tokens
@@ -264,7 +265,8 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
     ``cu_q`` row b is the one query of sequence b; with ``cu_q`` (int32 ``[B+1]``) rows ``cu_q[b]..cu_q[b+1]`` are the
     last tokens of sequence b, each seeing the tokens up to itself -- drafted tokens, a chunk of prompt.  A query that
     sees nothing gets zeros; rows behind ``cu_q[B]`` are not written.  Returns ``[T,Hq,D]`` in Q's dtype, or in that of
-    ``out`` (fp16 or bf16).  No reference counterpart.
+    ``out`` (fp16 or bf16).  A page-table entry outside the pool reads page 0 and sets ``SKV_DEV_BAD_PAGE`` (2) in ``status``
+    (an int32 device tensor of one element; without it, in the stream's workspace).  No reference counterpart.
     """
     bf16 = Q.dtype is torch.bfloat16
     _require(Q.is_cuda and (bf16 or Q.dtype is torch.float16) and Q.dim() == 3 and Q.is_contiguous(),
@@ -304,11 +306,15 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
         out_bf16 = out.dtype is torch.bfloat16
         _require((out_bf16 or out.dtype is torch.float16) and out.shape == Q.shape and out.is_contiguous()
                  and out.device == dev, "out must be a contiguous fp16 or bf16 tensor of Q's shape on Q's device")
+    if status is not None:
+        _require(status.dtype is torch.int32 and status.shape == (1,) and status.device == dev, "status must be an int32 [1] tensor on Q's device")
+        status = status.data_ptr()
     lib = _lib.load()
     stream = _workspace.stream(dev.index)
     ws = _workspace.scratch("gqa_kv4", lib.skv_gqa_decode_kv4_workspace_bytes(D), 8192, dev, stream)
     rc = lib.skv_gqa_decode_kv4(Q.data_ptr(), bf16, pool.data_ptr(), table, lens, cu, out.data_ptr(), out_bf16, ws.data_ptr(),
-                                ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages, sp, sh, scale, dev.index, stream)
+                                ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages, sp, sh, scale, status, dev.index,
+                                stream)
     if rc:
         _lib.check(rc, "fused_gqa_kv4")
     return out

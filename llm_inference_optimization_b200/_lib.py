@@ -76,7 +76,8 @@ SIGNATURES = {
     "skv_read_tokens": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                              _ll, _ll, _ll, _ll, _ll, _vp, _i, _vp]),
     "skv_gqa_decode_kv4_workspace_bytes": (_sz, [_i]),
-    "skv_gqa_decode_kv4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _f, _i, _vp]),
+    "skv_gqa_decode_kv4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _f, _vp,
+                                _i, _vp]),
     "skv_gqa_decode_noalloc_status": (_i, [_i, _vp, C.POINTER(_i)]),
     "skv_gqa_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _vp, _f, _i, _vp]),
 }

@@ -23,13 +23,17 @@
 //     N side; P goes from the one layout to the other by movmatrix.
 //
 // Streaming: every warp is on its own -- it copies records to a ring of its own with cp.async (16 bytes per lane and
-// request: two records are nine requests of a warp), keeps its own softmax state, and meets the others only at the end of a
+// request: a record is five requests of a warp), keeps its own softmax state, and meets the others only at the end of a
 // segment.  No producer warps and no barriers in the loop.
 //
 // Work split: the host does not know the lengths.  Work is counted in records over (kv-head, sequence, chunk of columns)
 // in this order and cut into equal runs, one for each CTA of ONE resident wave; a CTA finds its run with a scan of the
 // lengths and walks over the items in it.  An item that spans CTAs is summed by the last of them to finish (a ticket per
 // first CTA), in the order of the sequence: results do not depend on timing.
+//
+// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 65.9 us, 4.6 TB/s, 0.70 of a copy (the
+// stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 55 us; one of 4093 tokens
+// 11.8 us, all of it start, merge and sum.  ncu: issue slots 63 % busy, logic pipe 53 %, tensor pipe 27 %, DRAM half busy.
 #include <cuda_bf16.h>
 
 #include "skv_common.cuh"
@@ -42,24 +46,26 @@ namespace kv4 {
 // four powers of two before it moves again, and eleven bits for every weight down to 2^-24 of the largest.
 constexpr float WEIGHT_MAX = 14.f, WEIGHT_AIM = 10.f;
 constexpr float NOTHING = -1e30f;     // reference of a column that has seen no token
-constexpr int SETUP = 48;          // what starting an item costs a CTA, in records: query, first loads, merge
+// What starting an item costs a CTA, in records: query, first loads, merge.  (Without it CTAs with several items end last:
+// 16 ragged sequences 67.7 us with 0, 64.1 with 16, 62.4 with 48, 62.5 with 64 at the time it was brought in.)
+constexpr int SETUP = 48;
 constexpr int MIN_UNITS = 16;         // records per CTA at least: shorter runs are all start and end
 constexpr size_t TICKET_OFF = 256, PARTIAL_OFF = 8192;
 constexpr int MAX_GRID = 320;         // CTAs of one wave (a combine keeps this many (max, sum) pairs in registers)
 static_assert(MAX_GRID * 4 <= PARTIAL_OFF - TICKET_OFF, "tickets");
 
 template <int D, int NT> struct Shape {
-    static constexpr int NW = NT == 1 ? 6 : 8;           // warps per CTA: as many as the registers allow
+    static constexpr int NW = 8;                         // warps per CTA: sixteen an SM at 128 registers, eight at 256
     static constexpr int THREADS = NW * 32;
     static constexpr int W = D / 32;                     // scale groups per row
     static constexpr int REC = kv4_record_bytes<D>();
-    static constexpr int STAGES = 5;
+    static constexpr int STAGES = NT == 1 ? 3 : 5;       // records in a warp's ring: 55 | 92 KB of a CTA
     static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
-    static constexpr int ROW = D + 4;                    // merge rows, padded: 16-byte stores of a warp spread over the banks
+    static constexpr int ROW = D + 4;                    // rows of sums, padded: 16-byte stores of a warp spread over the banks
     static constexpr int RING = NW * STAGES * REC;
     static constexpr int MAX_N = MAX_GRID / (NT == 1 ? 1 : 2);                     // partial results of an item
     static constexpr int SCRATCH = MAX_N * 8 * NT * 4 + 16 * 4 + THREADS * 16 + 16;   // what combine() needs
-    static constexpr int TILE = NW * 8 * ROW * 4;        // one n-tile (8 columns) of every warp
+    static constexpr int TILE = NW * 8 * NT * ROW * 4;   // the sums of every warp
     static constexpr int MERGE = TILE > SCRATCH ? TILE : SCRATCH;
     static constexpr int ML = NW * 8 * NT * 8;           // (max, sum) per warp and column
     static constexpr int QUERY = NT * (W * 512 + 32 * 12);   // the item's columns as operands, and 12 bytes per lane
@@ -175,7 +181,7 @@ template <int D, int NC, int THREADS>
 __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n, int cols, int col0, float* scratch) {
     constexpr int REGS = (MAX_GRID / (NC / 8) + 31) / 32;
     constexpr int NW = THREADS / 32;
-    constexpr int U = 12;                               // partial rows in flight per thread
+    constexpr int U = 4;                                // partial rows in flight per thread (more would cost the loop registers)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* weight = scratch;                            // [n][cols]
     float* sums = scratch + ((n * cols + 3) & ~3);      // [cols]
@@ -357,14 +363,15 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_P
             page = p.page_table ? __ldg(p.page_table + (long long)seq * p.max_pages + r) : seq * p.max_pages + r;
         return checked_page(page, p.num_pages, bad_page);
     };
-    auto issue = [&](int k) {
+    auto issue = [&](int k, auto certain_constant) {  // (certain: the caller knows that record k exists)
+        constexpr bool CERTAIN = decltype(certain_constant)::value;
         if ((k & 31) == 0) {                          // pages of the next 32 records, one per lane, fetched 32 ahead
             const int r = r_first + (k + lane) * NW;
             page_now = k ? page_next : load_page(r);
             page_next = load_page(r + 32 * NW);
         }
         const int page = __shfl_sync(0xffffffffu, page_now, k & 31);
-        if (k < n_rec) {
+        if (CERTAIN || k < n_rec) {
             const uint8_t* src = head_base + (unsigned long long)(uint32_t)SKV_INDEX(page, p.num_pages) * p.sp;
             const uint32_t dst = ring + in_off + lane * 16;
 #pragma unroll
@@ -395,7 +402,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_P
         in_off = 0;
         head_base = p.pool + x.h * p.sh + lane * 16;
 #pragma unroll
-        for (int k = 0; k < STAGES - 1; ++k) issue(k);
+        for (int k = 0; k < STAGES - 1; ++k) issue(k, Constant<false>{});
     };
     begin(first, query);
 
@@ -513,7 +520,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_P
             constexpr bool MASKED = decltype(masked_constant)::value;
             cp_async_wait<STAGES - 2>();
             __syncwarp();                              // record k is here, and every lane is done with record k - 1
-            issue(k + STAGES - 1);
+            issue(k + STAGES - 1, Constant<!MASKED>{});
             const uint32_t rec = ring + out_off;
             out_off = out_off == (STAGES - 1) * REC ? 0 : out_off + REC;
             const int t0 = (r_first + k * NW) * 16 + tok_a;   // this lane's tokens: t0, t0 + 2
@@ -656,13 +663,36 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_P
                 }
             }
         };
-        // Records that every column sees whole, then those at the end, where columns differ.
+        // Records that every column sees whole, with another to fetch behind them; then those at the end.
         const int n_mine = n_rec;
         int k = 0;
-        for (; k < n_full; ++k) record(k, Constant<false>{});
+        for (; k < min(n_full, n_mine - (STAGES - 1)); ++k) record(k, Constant<false>{});
         for (; k < n_mine; ++k) record(k, Constant<true>{});
         cp_async_wait<0>();
         __syncwarp();
+
+        // ---- this warp's sums to shared memory (their registers are free then for what follows)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = nt * 8 + 2 * tq + j;
+                float l = lrun[nt][j];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                if (g == 0) merge_ml[warp * NC + c] = make_float2(ref[nt][j], l);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    // rows g hold (even + 16 odd) 2^-24, rows g + 8 odd 2^-20
+                    float4 v;
+                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * 16777216.f;
+                    v.y = o[nt][2 * w][j + 2] * 1048576.f;
+                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * 16777216.f;
+                    v.w = o[nt][2 * w + 1][j + 2] * 1048576.f;
+                    *reinterpret_cast<float4*>(merge + (warp * NC + c) * S::ROW + 32 * w + 4 * g) = v;
+                }
+            }
 
         // ---- the next segment's first records are on their way while this one is written
         const Segment done = state->sg;
@@ -684,60 +714,36 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_P
         if (more) begin(next, query + (~item & 1) * S::QUERY);
         const int col0 = done.chunk * NC, cols = min(done.s.nq * p.G - col0, NC);
 
-        // ---- merge the warps, a tile of 8 columns at a time
+        // ---- merge the warps
         const long long slot = 2ll * blockIdx.x + (done.r0 == 0 ? 1 : 0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < cols * (D / 4); i += THREADS) {
+            const int c = i / (D / 4), d = i % (D / 4) * 4;
+            float2 ml[NW];
+            float M = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int c = 2 * tq + j;
-                float l = lrun[nt][j];
-                l += __shfl_xor_sync(0xffffffffu, l, 4);
-                l += __shfl_xor_sync(0xffffffffu, l, 8);
-                l += __shfl_xor_sync(0xffffffffu, l, 16);
-                if (g == 0) merge_ml[warp * 8 + c] = make_float2(ref[nt][j], l);
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    // rows g hold (even + 16 odd) 2^-24, rows g + 8 odd 2^-20
-                    float4 v;
-                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * 16777216.f;
-                    v.y = o[nt][2 * w][j + 2] * 1048576.f;
-                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * 16777216.f;
-                    v.w = o[nt][2 * w + 1][j + 2] * 1048576.f;
-                    *reinterpret_cast<float4*>(merge + (warp * 8 + c) * S::ROW + 32 * w + 4 * g) = v;
-                }
+            for (int w = 0; w < NW; ++w) {
+                ml[w] = merge_ml[w * NC + c];
+                M = fmaxf(M, ml[w].x);
             }
-            __syncthreads();
-            const int n_cols = min(cols - nt * 8, 8);
-            for (int i = threadIdx.x; i < n_cols * (D / 4); i += THREADS) {
-                const int c = i / (D / 4), d = i % (D / 4) * 4;
-                float2 ml[NW];
-                float M = -INFINITY;
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    ml[w] = merge_ml[w * 8 + c];
-                    M = fmaxf(M, ml[w].x);
-                }
-                float L = 0.f;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float wt = fast_exp2(ml[w].x - M);
-                    const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + c) * S::ROW + d);
-                    L = fmaf(ml[w].y, wt, L);
-                    acc.x = fmaf(v.x, wt, acc.x); acc.y = fmaf(v.y, wt, acc.y);
-                    acc.z = fmaf(v.z, wt, acc.z); acc.w = fmaf(v.w, wt, acc.w);
-                }
-                const int col = nt * 8 + c;
-                if (done.whole) {
-                    store_out(p, done, D, col0 + col, d, acc, L);
-                } else {
-                    *reinterpret_cast<float4*>(p.partial_o + (slot * NC + col) * D + d) = acc;
-                    if (d == 0) *reinterpret_cast<float2*>(p.partial_ml + (slot * NC + col) * 2) = make_float2(M, L);
-                }
+            for (int w = 0; w < NW; ++w) {
+                const float wt = fast_exp2(ml[w].x - M);
+                const float4 v = *reinterpret_cast<const float4*>(merge + (w * NC + c) * S::ROW + d);
+                L = fmaf(ml[w].y, wt, L);
+                acc.x = fmaf(v.x, wt, acc.x); acc.y = fmaf(v.y, wt, acc.y);
+                acc.z = fmaf(v.z, wt, acc.z); acc.w = fmaf(v.w, wt, acc.w);
             }
-            __syncthreads();
+            if (done.whole) {
+                store_out(p, done, D, col0 + c, d, acc, L);
+            } else {
+                *reinterpret_cast<float4*>(p.partial_o + (slot * NC + c) * D + d) = acc;
+                if (d == 0) *reinterpret_cast<float2*>(p.partial_ml + (slot * NC + c) * 2) = make_float2(M, L);
+            }
         }
+        __syncthreads();
 
         // ---- an item that spans CTAs: the last one to arrive adds up
         if (!done.whole) {
@@ -779,7 +785,7 @@ static int launch(const Params& p, void* workspace, int device, cudaStream_t str
     if (grid > (units + MIN_UNITS - 1) / MIN_UNITS) grid = (units + MIN_UNITS - 1) / MIN_UNITS;
     Params q = p;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    q.status = reinterpret_cast<int*>(ws);
+    if (!q.status) q.status = reinterpret_cast<int*>(ws);
     q.tickets = reinterpret_cast<int*>(ws + TICKET_OFF);
     q.partial_ml = reinterpret_cast<float*>(ws + PARTIAL_OFF);
     q.partial_o = q.partial_ml + 2ll * MAX_GRID * 8 * 2;        // (NT = 2 has half the CTAs and twice the columns)
@@ -802,7 +808,7 @@ size_t skv_gqa_decode_kv4_workspace_bytes(int D) { return D == 64 || D == 128 ? 
 int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int* page_table, const int* seq_lens,
                        const int* cu_q, void* out, int out_is_bf16, void* workspace, size_t workspace_bytes, int T, int B, int N,
                        int Hq, int Hkv, int D, int max_pages, int num_pages, long long pool_stride_page,
-                       long long pool_stride_head, float scale, int device, void* stream) {
+                       long long pool_stride_head, float scale, int* status, int device, void* stream) {
     if (!pool) return fail(SKV_ERR_BAD_ARG, "skv_gqa_decode_kv4: null pool");
     if (T < 0 || B <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || num_pages <= 0 || max_pages <= 0)
         return fail(SKV_ERR_BAD_ARG, "skv_gqa_decode_kv4: sizes must be positive");
@@ -832,6 +838,7 @@ int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int
     p.B = B; p.T = T; p.N = N; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
     p.max_pages = max_pages; p.num_pages = num_pages; p.q_bf16 = q_is_bf16; p.out_bf16 = out_is_bf16;
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.status = status;
     // columns per pass over the cache: 8, or 16 where the (query token, head) pairs of a sequence fill more than 8
     const bool wide = (long long)p.G * ((T + B - 1) / B) > 8;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -249,9 +249,10 @@ class PagedKV4:
         return self.max_pages * 16
 
     def decode(self, Q: Tensor, scale: float, *, cu_q: Tensor | None = None, max_seq_len: int | None = None,
-               out: Tensor | None = None) -> Tensor:
+               out: Tensor | None = None, status: Tensor | None = None) -> Tensor:
         """Dense GQA attention over the whole cache, one or several query tokens per sequence (``_C.fused_gqa_kv4``)."""
-        return _C.fused_gqa_kv4(Q, self.buf, self.page_table, self.seq_lens, scale, cu_q=cu_q, max_seq_len=max_seq_len, out=out)
+        return _C.fused_gqa_kv4(Q, self.buf, self.page_table, self.seq_lens, scale, cu_q=cu_q, max_seq_len=max_seq_len, out=out,
+                                status=status)
 
 
 KV4_RECORD_ROWS = 18  # rows of D bytes per (page, head): 8 of key codes, 8 of value codes, 2 of bf16 scales

@@ -188,6 +188,14 @@ def test_bad_page_is_reported_and_others_untouched(cuda_device, bad):
         assert _workspace.status(ws) == 2 and torch.equal(got[0], want[0]) and torch.isfinite(got).all()
     finally:
         ws[:4].zero_()
+    word = torch.zeros(1, dtype=torch.int32, device=cuda_device)   # a word of the caller's, which a captured call can report to
+    q = c.q.to(cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.kv.decode(q, c.scale, status=word)
+    assert int(word) == 0
+    graph.replay()
+    assert int(word) == 2 and _workspace.status(ws) == 0
 
 
 def test_same_bits_every_time_and_on_other_streams(cuda_device):
@@ -295,6 +303,6 @@ def test_refusals(cuda_device):
                 lambda: call(t=c.kv.page_table.long()), lambda: call(n=c.kv.seq_lens[:1]), lambda: call(n=c.kv.seq_lens.cpu()),
                 lambda: call(s=0.0), lambda: call(s=float("nan")), lambda: call(max_seq_len=0), lambda: call(max_seq_len=33),
                 lambda: call(cu_q=cu[:2]), lambda: call(cu_q=cu.long()), lambda: call(out=torch.empty_like(q).float()),
-                lambda: call(out=torch.empty_like(q)[:1]), lambda: call(q=q.cpu()), lambda: call(t=None, pool=c.buf[:3])]:
+                lambda: call(out=torch.empty_like(q)[:1]), lambda: call(q=q.cpu()), lambda: call(status=torch.zeros(2, device=cuda_device)), lambda: call(t=None, pool=c.buf[:3])]:
         with pytest.raises(RuntimeError):
             bad()

@@ -86,7 +86,7 @@ def test_append_and_read_of_no_rows(lib):
 
 def attend_args(**kw):
     a = dict(q=16, bf16=0, pool=16, table=None, lens=None, cu=None, out=16, out_bf16=0, ws=256, nbytes=1 << 30, T=2, B=2, N=48, Hq=4, Hkv=2,
-             D=64, max_pages=3, pages=6, sp=2304, sh=1152, scale=0.125, dev=0, stream=None)
+             D=64, max_pages=3, pages=6, sp=2304, sh=1152, scale=0.125, status=None, dev=0, stream=None)
     assert set(kw) <= set(a)
     return list((a | kw).values())
 
@@ -95,7 +95,8 @@ def attend_args(**kw):
     (dict(pool=None), -1, "null pool"), (dict(q=None), -1, "null"), (dict(Hq=5), -1, "divisible"), (dict(D=32), -2, "head dims"),
     (dict(N=49), -1, "max_pages"), (dict(T=3), -1, "cu_q"), (dict(scale=0.0), -1, "scale"), (dict(nbytes=100), -3, "workspace"),
     (dict(ws=None), -3, "workspace"), (dict(ws=272), -3, "aligned"), (dict(pool=8), -1, "16 bytes"), (dict(sp=2300), -1, "16 bytes"),
-    (dict(q=8), -1, "16 bytes"), (dict(B=0), -1, "sizes"), (dict(Hkv=0), -1, "sizes")])
+    (dict(q=8), -1, "16 bytes"), (dict(B=0), -1, "sizes"), (dict(Hkv=0), -1, "sizes"), (dict(sp=1 << 33), -2, "stride"),
+    (dict(T=1 << 30, cu=16, Hq=16), -2, "rows")])
 def test_attention_refuses(lib, kw, code, word):
     assert lib.skv_gqa_decode_kv4(*attend_args(**kw)) == code
     assert word in _lib.last_error()
