@@ -1,7 +1,7 @@
 """Kernel-level sweep of the decode path on one B200: the counterpart of the reference's
 ``benchmarks/run_benchmarks.py`` (its 4K-128K sweep at B=1, H=32, D=128, :22-80) for the kernels here.
 
-    python -m llm_inference_optimization_b200.benchmarks [--only dense,paged,token,block,evict,quest] [--iters 20]
+    python -m llm_inference_optimization_b200.benchmarks [--only dense,paged,kv4,tokens,token,block,evict,quest] [--iters 20]
 
 Prints one JSON line per (workload, size): median CUDA-event time of the whole operator (all of its
 launches), the algorithmic bytes, GB/s and the fraction of the measured HBM copy bandwidth.  Inputs are
@@ -19,7 +19,7 @@ from pathlib import Path
 
 import torch
 
-from . import _C, eviction, paged
+from . import _C, eviction, paged, rotary
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -147,6 +147,47 @@ def bench_mixed(t, dev, g, peak, pk):
                                                                                   "layout": "mixed-precision page records"},
                  us, mn, nbytes, peak, pk, us_per_8bit_byte_count=round(us * 264 / 200, 2))
             del buf, kv
+
+
+def bench_kv4(t, dev, g, peak, pk):
+    """Dense decode over keys and values in 4 bits (144 bytes per token and head), one and several query tokens."""
+    Hq, Hkv, D = 32, 8, 128
+    for B, N, S in ((1, 4096, 1), (1, 65536, 1), (4, 65536, 1), (16, 65536, 1), (8, 16384, 4)):
+        pages = B * N // 16
+        buf = torch.randint(0, 256, (pages, Hkv, paged.KV4_RECORD_ROWS, D), device=dev, generator=g, dtype=torch.uint8)
+        buf[:, :, 16:].view(torch.bfloat16).copy_(torch.rand((pages, Hkv, 2, D // 2), device=dev, generator=g) * 0.2 + 0.3)
+        table = torch.randperm(pages, device=dev, generator=g).to(torch.int32).view(B, N // 16)
+        kv = paged.PagedKV4(buf, table, None, B)
+        Q = randn16((B * S, Hq, D), dev, g)
+        cu = None if S == 1 else torch.arange(B + 1, device=dev, dtype=torch.int32) * S
+        us, mn = t(lambda: kv.decode(Q, D ** -0.5, cu_q=cu))
+        emit("dense_gqa_paged_int4", {"B": B, "Hq": Hq, "Hkv": Hkv, "D": D, "ctx": N, "queries": S}, us, mn, B * N * Hkv * 144, peak, pk)
+        del buf, kv
+
+
+def bench_tokens(t, dev, g, peak, pk):
+    """Rotation of query and key rows, appending them to caches, reading tokens back: a step of 16 and a prompt of 8192."""
+    Hq, Hkv, D = 32, 8, 128
+    rope = rotary.RotaryEmbedding(D, 500000.0, device=dev)
+    for B, n in ((16, 1), (1, 8192)):
+        T = B * n
+        qkv = torch.randn((T, (Hq + 2 * Hkv) * D), device=dev, generator=g).bfloat16()
+        q, k = qkv.view(T, -1, D)[:, :Hq], qkv.view(T, -1, D)[:, Hq:Hq + Hkv]
+        pos = torch.arange(T, device=dev, dtype=torch.int32) % n
+        us, mn = t(lambda: rope.apply(pos, q, k))
+        emit("rotary", {"T": T, "Hq": Hq, "Hk": Hkv, "D": D}, us, mn, 2 * T * (Hq + Hkv) * D * 2, peak, pk)
+        cu = torch.arange(B + 1, device=dev, dtype=torch.int32) * n
+        lens = torch.full((B,), 100, device=dev, dtype=torch.int32)
+        pages = (n + 100 + 15) // 16
+        for name, rows, width, make in (("int4", paged.KV4_RECORD_ROWS, 144, paged.PagedKV4),
+                                        ("fp8", paged.RECORD_ROWS, 264, lambda b, *a: paged.PagedKV.from_fused(b, torch.float8_e4m3fn, *a))):
+            buf = torch.zeros((B * pages, Hkv, rows, 128), dtype=torch.uint8, device=dev)
+            kv = make(buf, torch.randperm(B * pages, device=dev, generator=g).to(torch.int32).view(B, pages), lens, B)
+            cfg = {"T": T, "B": B, "Hq": Hq, "Hkv": Hkv, "D": D, "cache": name}
+            us, mn = t(lambda: paged.append_tokens(qkv, kv, Hq, rope, cu_new=cu))
+            emit("append_tokens", cfg, us, mn, T * ((Hq + 2 * Hkv) * D * 2 + Hq * D * 2 + Hkv * width), peak, pk)
+            us, mn = t(lambda: paged.read_tokens(kv, cu, T, starts=lens))
+            emit("read_tokens", cfg, us, mn, T * Hkv * (width + 4 * D), peak, pk)
 
 
 def bench_paged_stream(t, dev, g, peak, pk):
@@ -289,7 +330,7 @@ def bench_quest(t, dev, g, peak, pk):
          us, mn, nbytes, peak, pk)
 
 
-ALL = {"dense": bench_dense, "paged": bench_paged, "mixed": bench_mixed, "paged_stream": bench_paged_stream, "ragged": bench_ragged, "token": bench_token, "block": bench_block, "evict": bench_evict,
+ALL = {"dense": bench_dense, "paged": bench_paged, "mixed": bench_mixed, "kv4": bench_kv4, "tokens": bench_tokens, "paged_stream": bench_paged_stream, "ragged": bench_ragged, "token": bench_token, "block": bench_block, "evict": bench_evict,
        "quest": bench_quest}
 
 
