@@ -31,7 +31,7 @@
 // lengths and walks over the items in it.  An item that spans CTAs is summed by the last of them to finish (a ticket per
 // first CTA), in the order of the sequence: results do not depend on timing.
 //
-// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 65.9 us, 4.6 TB/s, 0.70 of a copy (the
+// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 63.9 us, 4.7 TB/s, 0.72 of a copy (the
 // stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 55 us; one of 4093 tokens
 // 11.8 us, all of it start, merge and sum.  ncu: issue slots 63 % busy, logic pipe 53 %, tensor pipe 27 %, DRAM half busy.
 #include <cuda_bf16.h>
@@ -46,25 +46,26 @@ namespace kv4 {
 // four powers of two before it moves again, and eleven bits for every weight down to 2^-24 of the largest.
 constexpr float WEIGHT_MAX = 14.f, WEIGHT_AIM = 10.f;
 constexpr float NOTHING = -1e30f;     // reference of a column that has seen no token
-// What starting an item costs a CTA, in records: query, first loads, merge.  (Without it CTAs with several items end last:
-// 16 ragged sequences 67.7 us with 0, 64.1 with 16, 62.4 with 48, 62.5 with 64 at the time it was brought in.)
-constexpr int SETUP = 48;
 constexpr int MIN_UNITS = 16;         // records per CTA at least: shorter runs are all start and end
 constexpr size_t TICKET_OFF = 256, PARTIAL_OFF = 8192;
-constexpr int MAX_GRID = 320;         // CTAs of one wave (a combine keeps this many (max, sum) pairs in registers)
+constexpr int MAX_GRID = 160;         // CTAs of one wave (a combine keeps this many (max, sum) pairs in a warp's registers)
 static_assert(MAX_GRID * 4 <= PARTIAL_OFF - TICKET_OFF, "tickets");
 
 template <int D, int NT> struct Shape {
-    static constexpr int NW = 8;                         // warps per CTA: sixteen an SM at 128 registers, eight at 256
+    // Warps of a CTA, one CTA an SM: 16 at 128 registers, 8 at 256.  (Two CTAs of 8: the one that came first on its SM ended
+    // at 50 us of 4 sequences of 65536 tokens, the other at 62; 16 warps of one end within 3 us of one another, at 60.)
+    static constexpr int NW = NT == 1 ? 16 : 8;
+    // What starting an item costs a CTA, in records its warps could have read: query, first loads, merge.  (Without it CTAs
+    // with several items end last: 16 ragged sequences 67.7 us with 0, 64.1 with a third, 62.4 with this, 62.5 with four
+    // thirds at the time it was brought in.)
+    static constexpr int SETUP = 6 * NW;
     static constexpr int THREADS = NW * 32;
     static constexpr int W = D / 32;                     // scale groups per row
     static constexpr int REC = kv4_record_bytes<D>();
-    static constexpr int STAGES = NT == 1 ? 3 : 5;       // records in a warp's ring: 55 | 92 KB of a CTA
-    static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
+    static constexpr int STAGES = NT == 1 ? 3 : 5;       // records in a warp's ring: 111 | 92 KB of a CTA at D = 128
     static constexpr int ROW = D + 4;                    // rows of sums, padded: 16-byte stores of a warp spread over the banks
     static constexpr int RING = NW * STAGES * REC;
-    static constexpr int MAX_N = MAX_GRID / (NT == 1 ? 1 : 2);                     // partial results of an item
-    static constexpr int SCRATCH = MAX_N * 8 * NT * 4 + 16 * 4 + THREADS * 16 + 16;   // what combine() needs
+    static constexpr int SCRATCH = MAX_GRID * 8 * NT * 4 + 16 * 4 + THREADS * 16 + 16;   // what combine() needs
     static constexpr int TILE = NW * 8 * NT * ROW * 4;   // the sums of every warp
     static constexpr int MERGE = TILE > SCRATCH ? TILE : SCRATCH;
     static constexpr int ML = NW * 8 * NT * 8;           // (max, sum) per warp and column
@@ -179,7 +180,7 @@ __device__ __forceinline__ void store_out(const Params& p, const Segment& x, int
 // threads are split over the partials where the columns leave them free; every sum has one order, whoever runs it.
 template <int D, int NC, int THREADS>
 __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n, int cols, int col0, float* scratch) {
-    constexpr int REGS = (MAX_GRID / (NC / 8) + 31) / 32;
+    constexpr int REGS = (MAX_GRID + 31) / 32;
     constexpr int NW = THREADS / 32;
     constexpr int U = 4;                                // partial rows in flight per thread (more would cost the loop registers)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -262,9 +263,10 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__((Shape<D, NT>::THREADS), (Shape<D, NT>::CTAS_PER_SM)) gqa_decode_kv4_kernel(const Params p) {
+__global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_kernel(const Params p) {
     using S = Shape<D, NT>;
     constexpr int W = S::W, NC = 8 * NT, REC = S::REC, STAGES = S::STAGES, NW = S::NW, THREADS = S::THREADS;
+    constexpr int SETUP = S::SETUP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -779,22 +781,21 @@ static int launch(const Params& p, void* workspace, int device, cudaStream_t str
     }
     // no more CTAs than the longest possible work gives MIN_UNITS records each
     const long long chunks = ((long long)p.T * p.G + NC - 1) / NC + (p.cu_q ? p.B : 0);
-    const long long units = p.Hkv * (p.cu_q ? chunks : (long long)p.B * ((p.G + NC - 1) / NC)) * (SETUP + ((long long)p.N + 15) / 16);
-    long long grid = (long long)sm_count(device) * S::CTAS_PER_SM;
-    if (grid > S::MAX_N) grid = S::MAX_N;
+    const long long units = p.Hkv * (p.cu_q ? chunks : (long long)p.B * ((p.G + NC - 1) / NC)) * (S::SETUP + ((long long)p.N + 15) / 16);
+    long long grid = sm_count(device) < MAX_GRID ? sm_count(device) : MAX_GRID;
     if (grid > (units + MIN_UNITS - 1) / MIN_UNITS) grid = (units + MIN_UNITS - 1) / MIN_UNITS;
     Params q = p;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     if (!q.status) q.status = reinterpret_cast<int*>(ws);
     q.tickets = reinterpret_cast<int*>(ws + TICKET_OFF);
     q.partial_ml = reinterpret_cast<float*>(ws + PARTIAL_OFF);
-    q.partial_o = q.partial_ml + 2ll * MAX_GRID * 8 * 2;        // (NT = 2 has half the CTAs and twice the columns)
+    q.partial_o = q.partial_ml + 2ll * MAX_GRID * NC * 2;
     SKV_CUDA_TRY(launch_pdl(gqa_decode_kv4_kernel<D, NT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, stream, q));
     SKV_CUDA_TRY(cudaGetLastError());
     return SKV_OK;
 }
 
-static size_t workspace_bytes(int D) { return PARTIAL_OFF + 2ull * MAX_GRID * 8 * (2 + D) * 4; }
+static size_t workspace_bytes(int D) { return PARTIAL_OFF + 2ull * MAX_GRID * 16 * (2 + D) * 4; }   // 16 columns: NT = 2
 
 }  // namespace kv4
 }  // namespace skv
