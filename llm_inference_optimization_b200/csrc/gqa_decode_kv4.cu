@@ -31,9 +31,9 @@
 // lengths and walks over the items in it.  An item that spans CTAs is summed by the last of them to finish (a ticket per
 // first CTA), in the order of the sequence: results do not depend on timing.
 //
-// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 63.9 us, 4.7 TB/s, 0.72 of a copy (the
-// stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 55 us; one of 4093 tokens
-// 11.8 us, all of it start, merge and sum.  ncu: issue slots 63 % busy, logic pipe 53 %, tensor pipe 27 %, DRAM half busy.
+// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 63.3 us, 4.8 TB/s, 0.73 of a copy (the
+// stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 54.6 us; one of 4093 tokens
+// 11.7 us, all of it start, merge and sum.  ncu: issue slots 63 % busy, logic pipe 53 %, tensor pipe 27 %, DRAM half busy.
 #include <cuda_bf16.h>
 
 #include "skv_common.cuh"
@@ -288,13 +288,27 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
 
     // ---- this CTA's run of the work list (every warp finds it for itself).  An item counts SETUP units for starting it and
     // one for each record; positions fit 32 bits but for work of days, whose runs are found in 64.
-    long long per_head = 0;
-    for (int b = lane; b < p.B; b += 32) {
-        const Seq s = sequence<NC>(p, b);
-        per_head += (long long)s.chunks * (SETUP + s.recs);
-    }
+    auto units = [&](int b) {                         // of sequence b + lane of a kv-head
+        if (b + lane >= p.B) return 0ll;
+        const Seq s = sequence<NC>(p, b + lane);
+        return (long long)s.chunks * (SETUP + s.recs);
+    };
+    auto prefix = [&](long long v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, o);
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        return v;
+    };
+    long long mine = units(0), upto = prefix(mine);   // the first 32 sequences, of most calls all: counted once
+    long long per_head = 0;
+    for (int b0 = 32; b0 < p.B; b0 += 32) per_head += units(b0);
+    if (p.B > 32) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, o);
+    }
+    per_head += __shfl_sync(0xffffffffu, upto, 31);
     const long long total = per_head * p.Hkv;
     const bool small = total < 0x40000000ll;
     auto divide = [&](long long a, long long b) { return small ? (long long)((uint32_t)a / (uint32_t)b) : a / b; };
@@ -325,16 +339,9 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
         long long rest = at - sg.h * per_head;
         sg.b = -1;
         for (int b0 = 0; b0 < p.B; b0 += 32) {        // find the sequence: a warp-wide prefix sum of 32 at a time
-            long long mine = 0;
-            if (b0 + lane < p.B) {
-                const Seq s = sequence<NC>(p, b0 + lane);
-                mine = (long long)s.chunks * (SETUP + s.recs);
-            }
-            long long upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
+            if (b0 > 0) {
+                mine = units(b0);
+                upto = prefix(mine);
             }
             const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
             if (past) {
