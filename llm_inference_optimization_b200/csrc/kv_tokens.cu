@@ -222,8 +222,12 @@ __device__ __forceinline__ int page_of(const Pools& c, int b, long long pos, int
     return SKV_INDEX(page, c.num_pages);
 }
 
-// 8192 tokens, 32 + 8 + 8 heads of 128 in bf16, 4-bit cache: 42.5 us (4.2 TB/s, 0.64 of a copy; 37.9 without rotation).  Bound by
-// instructions, 160 per two rows at two thirds of the issue slots; U and registers of 2 | 64, 3 | 80, 4 | 96: 43.4, 42.5, 43.9.
+// 8192 tokens, 32 + 8 + 8 heads of 128 in bf16, 4-bit cache: 42.5 us (4.2 TB/s, 0.64 of a copy; 37.9 without rotation).  No one
+// limit shows: issue slots are 70 % busy (163 instructions per two rows), waits are for fixed latencies, shared memory and
+// instructions more than for loads, and a copy without what a block finds out first (sequence, length, page, sines) takes
+// 37.3.  Query rows as four channels and their four partners, without shuffles: 45.0; with loops of their own for query rows
+// and for keys and values: 43.7 at best, and narrow rows slower (5.9 -> 6.6).  U and registers of 2 | 64, 3 | 80, 4 | 96: 43.4, 42.5, 43.9;
+// blocks of 64, 96, 256 threads: 44.6, 45.1, 53.6; plain loads 43.0.
 template <typename T, int D, int CACHE>
 __global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendParams p) {
     constexpr int LPR = D / 8, U = 3;

@@ -203,7 +203,9 @@ __global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) 
                 } else {
                     *reinterpret_cast<V*>(d) = lo;
                 }
-                if (!INTER && turned) *reinterpret_cast<V*>(d + p.R / 2) = hi;
+                if constexpr (!INTER) {
+                    if (turned) *reinterpret_cast<V*>(d + p.R / 2) = hi;
+                }
             }
         }
     }
