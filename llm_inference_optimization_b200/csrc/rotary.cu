@@ -264,6 +264,15 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
     if (rotary_dim <= 0 || rotary_dim > D || rotary_dim % 2)
         return fail(SKV_ERR_BAD_ARG, "skv_rotary: rotary_dim %d must be even and in 2..%d", rotary_dim, D);
     if (dtype < 0 || dtype > 2) return fail(SKV_ERR_UNSUPPORTED, "skv_rotary: dtype %d is not fp16, bf16 or fp32", dtype);
+    // Rows that share memory would be turned by several threads at once: views with a repeated or shortened stride as
+    // destination (an expanded tensor rotated in place), or one destination for both.
+    auto overlaps = [&](int H, long long dt, long long dh) {
+        const long long a = dt < 0 ? -dt : dt, b = dh < 0 ? -dh : dh;
+        return (T > 1 && a < D) || (H > 1 && b < D) || (T > 1 && H > 1 && a == b);
+    };
+    if ((Hq && overlaps(Hq, q_out_stride_t, q_out_stride_h)) || (Hk && overlaps(Hk, k_out_stride_t, k_out_stride_h)) ||
+        (Hq && Hk && q_out == k_out))
+        return fail(SKV_ERR_BAD_ARG, "skv_rotary: rows of the outputs overlap");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(SKV_ERR_CUDA, "cannot switch to device %d", device);
     rot::Params p;

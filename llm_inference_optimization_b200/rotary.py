@@ -101,7 +101,7 @@ class RotaryEmbedding:
         """Rotate ``q [T,Hq,D]`` (and ``k [T,Hk,D]``) at ``positions [T]`` (int32 or int64) in one launch.
 
         fp16, bf16 or fp32 (both alike; arithmetic in fp32), any strides with contiguous channels, for example slices of a
-        fused projection.  Returns new contiguous tensors, or the inputs with ``inplace``.  ``adjoint`` applies the
+        fused projection.  Returns new contiguous tensors, or the inputs with ``inplace`` (whose rows must not share memory).  ``adjoint`` applies the
         transposed map: given gradients of the outputs it returns those of the inputs.  No autograd graph is recorded, and
         inputs that would need one are refused."""
         _C._require(q.is_cuda and q.dim() == 3 and q.dtype in _DTYPES, "q must be an fp16, bf16 or fp32 CUDA tensor [T,H,head_dim]")

@@ -79,3 +79,12 @@ def test_entry_point_argument_errors(lib):
     assert lib.skv_rotary(16, None, 16, None, 0, 16, 0, 16, -1, 2, 0, 64, 64, 0, 1.0, 0, *z, 0, None) == -1
     assert lib.skv_rotary(None, None, None, None, 0, None, 0, None, 0, 2, 0, 64, 64, 0, 1.0, 0, *z, 0, None) == 0    # no rows
     assert hasattr(skv, "rotary")
+
+
+@pytest.mark.parametrize("q, k", [((0, 64), None), ((128, 0), None), ((32, 256), None), ((64, 64), None), ((128, 64), (0, 64)),
+                                  ((128, 64), (128, 32)), ((128, 64), "same")])
+def test_outputs_that_overlap_are_refused(lib, q, k):
+    """Expanded or shortened strides, or one destination for both, of four tokens and two heads: before any launch."""
+    kp, Hk, ks = (None, 0, (0, 0)) if k is None else (4096, 2, (128, 64)) if k == "same" else (1 << 20, 2, k)
+    assert lib.skv_rotary(4096, kp, 4096, kp, 0, 16, 0, 16, 4, 2, Hk, 64, 64, 0, 1.0, 0, *q, *ks, *q, *ks, 0, None) == -1
+    assert "overlap" in _lib.last_error()
