@@ -414,11 +414,15 @@ class DecodeModel:
     def extend(self, tokens: Tensor, cu_new: Tensor) -> Tensor:
         """Take any number of new tokens per sequence: a prompt, a chunk of one, drafted tokens to be checked.
 
-        ``tokens [T]`` int64, sequence b's new ones at ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``, ``cu_new[B] == T``); each
-        attends to its sequence up to itself.  Returns logits ``[T, vocab]`` and advances ``seq_lens`` by the counts
-        (a caller that rejects drafted tokens subtracts them again).  Models with 4-bit keys and values on a GPU."""
+        ``tokens [T]`` int64, sequence b's new ones at ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``); each attends to its sequence
+        up to itself.  Returns logits ``[T, vocab]`` and advances ``seq_lens`` by the counts (a caller that rejects drafted
+        tokens subtracts them again).  Tokens behind ``cu_new[B]`` are padding: nothing is stored for them and their logits mean
+        nothing.  The cache must have room for the new tokens (``init_cache(extra_tokens=)``), as for :meth:`step`.  Models with
+        4-bit keys and values on a GPU."""
         if not (self.fused_glue and self.k_bits == 4):
             raise RuntimeError("extend needs the CUDA glue path and a cache of 4-bit keys and values (k_bits=4, v_bits=4)")
+        if tokens.shape[0] == 0:
+            return self._logits(self.embed[tokens])
         counts = cu_new[1:] - cu_new[:-1]
         new_lens = self.seq_lens + counts
         h = self._fused_layers(self.embed[tokens], self.seq_lens, new_lens, 1.0 / math.sqrt(self.cfg.D), cu_new)

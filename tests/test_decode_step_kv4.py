@@ -125,3 +125,41 @@ def test_step_replays_from_a_graph(cuda_device):
     want = m.step(tok)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and math.isfinite(float(got.float().sum()))
+
+
+@pytest.mark.gpu
+def test_padded_and_empty_prompts(cuda_device):
+    """Tokens behind the last sequence change nothing for the others, in logits (up to roundings of matrix products of another
+    shape) and lengths, nor is anything stored for a sequence without new ones; no tokens at all give no logits and leave the lengths."""
+    toks = torch.randint(0, 512, (24,), generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    plain, padded = (ds.DecodeModel(CFG, shard_heads(8, 2, 1, 0), cuda_device, dtype=torch.bfloat16, v_bits=4, k_bits=4) for _ in range(2))
+    for m in (plain, padded):
+        m.init_cache(torch.zeros(3, dtype=torch.int32), fill="zeros", extra_tokens=64)
+    cu = offsets([9, 0, 11]).to(cuda_device)
+    a, b = plain.extend(toks[:20], cu), padded.extend(toks, cu)
+    assert b.shape == (24, 512) and near(b[:20], a, 12)
+    assert plain.seq_lens.tolist() == padded.seq_lens.tolist() == [9, 0, 11]
+    untouched = padded.page_table[1].long()
+    assert not any(c.buf[untouched].any() for c in padded.caches)
+    none = padded.extend(toks[:0], offsets([0, 0, 0]).to(cuda_device))
+    assert none.shape == (0, 512) and padded.seq_lens.tolist() == [9, 0, 11]
+
+
+@pytest.mark.gpu
+def test_prompt_replays_from_a_graph(cuda_device):
+    m = ds.DecodeModel(CFG, shard_heads(8, 2, 1, 0), cuda_device, dtype=torch.bfloat16, v_bits=4, k_bits=4)
+    m.init_cache(LENS, extra_tokens=64)
+    toks = torch.randint(0, 512, (13,), generator=torch.Generator().manual_seed(3)).to(cuda_device)
+    cu = offsets([4, 1, 8]).to(cuda_device)
+    m.extend(toks, cu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.extend(toks, cu)
+    m.seq_lens.copy_(LENS)
+    graph.replay()
+    got = out.clone()
+    m.seq_lens.copy_(LENS)
+    want = m.extend(toks, cu)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
