@@ -847,8 +847,11 @@ int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int
     p.max_pages = max_pages; p.num_pages = num_pages; p.q_bf16 = q_is_bf16; p.out_bf16 = out_is_bf16;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = status;
-    // columns per pass over the cache: 8, or 16 where the (query token, head) pairs of a sequence fill more than 8
-    const bool wide = (long long)p.G * ((T + B - 1) / B) > 8;
+    // Columns per pass over the cache, 8 or 16.  A pass of 16 takes 7/4 of one of 8, so it pays where it saves that many of the
+    // mean sequence's (query token, head) pairs' passes.  Measured with 8 | 16, D = 128, us: 16 pairs of 8 sequences of 8192
+    // tokens 42.5 | 39.9, 24 pairs 57.1 | 62.0, 32 pairs 71.6 | 63.5; 512 of one of 4096 76.2 | 65.7.
+    const long long pairs = (long long)p.G * ((T + B - 1) / B);
+    const bool wide = 7 * ((pairs + 15) / 16) < 4 * ((pairs + 7) / 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (D == 128) return wide ? kv4::launch<128, 2>(p, workspace, device, st) : kv4::launch<128, 1>(p, workspace, device, st);
     return wide ? kv4::launch<64, 2>(p, workspace, device, st) : kv4::launch<64, 1>(p, workspace, device, st);
