@@ -307,14 +307,15 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
         out_bf16 = out.dtype is torch.bfloat16
         _require((out_bf16 or out.dtype is torch.float16) and out.shape == Q.shape and out.is_contiguous()
                  and out.device == dev, "out must be a contiguous fp16 or bf16 tensor of Q's shape on Q's device")
+    word = None
     if status is not None:
         _require(status.dtype is torch.int32 and status.shape == (1,) and status.device == dev, "status must be an int32 [1] tensor on Q's device")
-        status = status.data_ptr()
+        word = status.data_ptr()
     lib = _lib.load()
     stream = _workspace.stream(dev.index)
     ws = _workspace.scratch("gqa_kv4", lib.skv_gqa_decode_kv4_workspace_bytes(D), 8192, dev, stream)
     rc = lib.skv_gqa_decode_kv4(Q.data_ptr(), bf16, pool.data_ptr(), table, lens, cu, out.data_ptr(), out_bf16, ws.data_ptr(),
-                                ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages, sp, sh, scale, status, dev.index,
+                                ws.numel(), T, B, N, Hq, Hkv, D, max_pages, num_pages, sp, sh, scale, word, dev.index,
                                 stream)
     if rc:
         _lib.check(rc, "fused_gqa_kv4")

@@ -320,6 +320,8 @@ def _token_cache(kv):
 
 
 def _int32(t: Tensor, n: int, dev, what: str) -> int:
+    """Pointer of an int32 argument.  The caller keeps the tensor under its own name until the launch: one made in the call would
+    else be freed here, and its memory given to the outputs that are allocated next."""
     if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == dev):
         raise RuntimeError(f"{what} must be a contiguous int32 [{n}] tensor on the cache's device")
     return t.data_ptr()
@@ -347,17 +349,18 @@ def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, 
     T, B = qkv.shape[0], kv.batch
     _C._require(kv.seq_lens is not None, "the cache needs seq_lens")
     lens = _int32(kv.seq_lens, B, dev, "seq_lens")
+    cu = pos = None
     if cu_new is None:
         _C._require(T == B, "one row per sequence, or cu_new")
     else:
-        cu_new = _int32(cu_new, B + 1, dev, "cu_new")
+        cu = _int32(cu_new, B + 1, dev, "cu_new")
     freqs, width, inter, factor = (None, 0, 0, 1.0) if rope is None else rope.kernel_args(D, dev)
     pos64 = False
     if positions is not None:
         pos64 = positions.dtype is torch.int64
         _C._require((pos64 or positions.dtype is torch.int32) and positions.shape == (T,) and positions.is_contiguous()
                     and positions.device == dev, "positions must be a contiguous int32 or int64 [T] tensor on the cache's device")
-        positions = positions.data_ptr()
+        pos = positions.data_ptr()
     if q_out is None:
         q_out, q_bf16 = qkv.new_empty((T, Hq, D), dtype=torch.float16), False
     else:
@@ -366,7 +369,7 @@ def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, 
                     and q_out.device == dev, "q_out must be a contiguous fp16 or bf16 [T,Hq,D] tensor on the cache's device")
     rc = _lib.load().skv_append_tokens(
         qkv.data_ptr(), bf16, qkv.stride(0) if T > 1 else qkv.shape[1], q_out.data_ptr(), q_bf16, freqs, width, inter, factor,
-        positions, pos64, cu_new, table, lens, *pools, T, B, Hq, Hkv, D, *layout,
+        pos, pos64, cu, table, lens, *pools, T, B, Hq, Hkv, D, *layout,
         None if status is None else _int32(status, 1, dev, "status"), dev.index, _workspace.stream(dev.index))
     if rc:
         _lib.check(rc, "append_tokens")
@@ -384,11 +387,11 @@ def read_tokens(kv: "PagedKV | PagedKV4", cu: Tensor, rows: int, *, starts: Tens
     pools, layout, table, Hkv, D, dev = _token_cache(kv)
     _C._require((dtype is torch.float16 or dtype is torch.bfloat16) and rows >= 0, "read_tokens returns fp16 or bf16 rows")
     B = kv.batch
-    cu = _int32(cu, B + 1, dev, "cu")
+    offsets = _int32(cu, B + 1, dev, "cu")
     K = torch.empty((rows, Hkv, D), dtype=dtype, device=dev)
     V = torch.empty_like(K)
     rc = _lib.load().skv_read_tokens(
-        *pools, table, cu, None if starts is None else _int32(starts, B, dev, "starts"), K.data_ptr(), V.data_ptr(),
+        *pools, table, offsets, None if starts is None else _int32(starts, B, dev, "starts"), K.data_ptr(), V.data_ptr(),
         dtype is torch.bfloat16, rows, B, Hkv, D, *layout, None if status is None else _int32(status, 1, dev, "status"),
         dev.index, _workspace.stream(dev.index))
     if rc:
