@@ -227,13 +227,14 @@ int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype
  *   heads, v heads) belongs to the sequence b with cu_new[b] <= t < cu_new[b + 1] (cu_new: int32 [B + 1]; NULL: row b to
  *   sequence b, T = B) and takes position seq_lens[b] + t - cu_new[b] of it.  q and k are rotated as by skv_rotary
  *   (rope_freqs NULL: not at all) at that position, or at positions[t] when given; q goes to q_out [T, Hq, D] (fp16, or
- *   bf16 with q_out_is_bf16), k and v are quantised and stored.  Rows behind cu_new[B] are left alone, in q_out too.
+ *   bf16 with q_out_is_bf16), k and v are quantised and stored.  Rows before cu_new[0] and from cu_new[B] on belong to no
+ *   sequence and are left alone, in q_out too.
  *   seq_lens is not modified.  A position past max_pages * page_size stores nothing, nor does one whose page-table entry
  *   lies outside [0, num_pages), which sets SKV_DEV_BAD_PAGE in *status (optional).  A row (4-bit: a group of 32
  *   channels) that is not finite is stored with scale NaN.  rotary_dim is a multiple of 16 (interleaved: of 8).
  * skv_read_tokens: row t with cu[b] <= t < cu[b + 1] receives the token at position starts[b] + t - cu[b] (starts NULL: 0)
  *   of sequence b as values, k_out / v_out [T, Hkv, D] fp16 (bf16 with out_is_bf16), code * scale rounded once; zeros where
- *   the cache has no page.  Rows behind cu[B] are left alone.
+ *   the cache has no page.  Rows before cu[0] and from cu[B] on are left alone.
  * Caches (kv_dtype): SKV_KV_I8 or SKV_KV_E4M3, with SKV_V_INT4 for 4-bit values, pools and strides as for
  *   skv_rope_quant_append (D = 128, rows 16-byte aligned); SKV_KV_INT4: k_pool = base of the records, strides of page and
  *   head in bytes, the other pool arguments unused (D = 64 or 128, page_size 16). */
@@ -260,7 +261,7 @@ int skv_read_tokens(const void* k_pool, const void* v_pool, const float* k_scale
  *   scales  bf16 element at byte 16D + place * D/8 + 2w (keys), + D/16 (values), group w < D/32
  * q, out: [T, Hq, D], fp16 or bf16 each.  cu_q int32 [B + 1]: rows cu_q[b] .. cu_q[b + 1] are the last query tokens of
  * sequence b, query i of n sees positions < seq_lens[b] - n + i + 1 (none: zeros); NULL: one query per sequence, T = B.
- * Rows behind cu_q[B] of out are left alone.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
+ * Rows before cu_q[0] and from cu_q[B] on are left alone in out.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
  * skv_gqa_decode_paged.  pool strides in bytes.  D = 64 or 128, any Hq / Hkv.  The result does not depend on timing.
  * A page-table entry outside [0, num_pages) reads page 0 and sets SKV_DEV_BAD_PAGE in *status (optional int32 device word;
  * NULL: the workspace's, at offset 0).  Workspace: skv_gqa_decode_kv4_workspace_bytes(D); its first 8192 bytes are zero

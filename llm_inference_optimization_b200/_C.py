@@ -264,7 +264,7 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
     sequence b owns pages ``b*max_pages ...``); ``seq_lens`` int32 ``[B]`` (``None``: every sequence is full).  Without
     ``cu_q`` row b is the one query of sequence b; with ``cu_q`` (int32 ``[B+1]``) rows ``cu_q[b]..cu_q[b+1]`` are the
     last tokens of sequence b, each seeing the tokens up to itself -- drafted tokens, a chunk of prompt.  A query that
-    sees nothing gets zeros; rows behind ``cu_q[B]`` are not written.  Lengths count up to ``max_seq_len`` (the page list's
+    sees nothing gets zeros; rows before ``cu_q[0]`` and from ``cu_q[B]`` on are not written.  Lengths count up to ``max_seq_len`` (the page list's
     room unless given): what lies behind it is not there, and the last query is then the one at its end.  Returns ``[T,Hq,D]`` in Q's dtype, or in that of
     ``out`` (fp16 or bf16).  A page-table entry outside the pool reads page 0 and sets ``SKV_DEV_BAD_PAGE`` (2) in ``status``
     (an int32 device tensor of one element; without it, in the stream's workspace).  No reference counterpart.

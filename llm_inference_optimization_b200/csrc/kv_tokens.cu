@@ -56,7 +56,8 @@ struct ReadParams {
 };
 
 // Sequence of row t: the number of sequences that end at or before it (B: behind the last).  Lanes of a row share the
-// count while a few loads each do it, else they all search.  An array that does not ascend gives some sequence: the row's
+// count while a few loads each do it, else they all search.  Whether the row is that sequence's is the caller's question: offsets
+// that begin above 0 give the rows before them sequence 0.  An array that does not ascend gives some sequence: the row's
 // position is checked before anything is stored.
 template <int LPR>
 __device__ __forceinline__ int sequence_of(const int* cu, int B, long long t, int l, unsigned group) {
@@ -260,10 +261,14 @@ __global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendP
         const int s = sequence_of<LPR>(p.cu_new, p.B, in ? t : (long long)p.T, l, group);
         b = in ? s : p.B;
     }
-    const bool mine = b < p.B;               // rows behind the last sequence are left alone
     int page = -1, slot = 0;
+    bool mine = b < p.B;                     // rows before the first sequence and behind the last are left alone
     if (mine) {
-        pos = (long long)p.seq_lens[b] + (p.cu_new ? t - p.cu_new[b] : 0);
+        const long long i = p.cu_new ? t - p.cu_new[b] : 0;
+        mine = i >= 0;
+        pos = (long long)p.seq_lens[b] + i;
+    }
+    if (mine) {
         page = page_of(p.c, b, pos, slot);
         if (p.positions) pos = p.pos64 ? static_cast<const long long*>(p.positions)[t]
                                        : (long long)static_cast<const int*>(p.positions)[t];
@@ -395,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) read_tokens_kernel(const ReadParams p
     const long long t = (long long)(warp / (unsigned)p.head_splits) * (32 / LPR) + lane / LPR;
     const bool in = t < p.T;
     const int s = sequence_of<LPR>(p.cu, p.B, in ? t : (long long)p.T, l, 0xffffffffu);
-    if (!in || s >= p.B) return;             // rows behind the last sequence are left alone
+    if (!in || s >= p.B || t < p.cu[s]) return;   // rows before the first sequence and behind the last are left alone
     int slot = 0;
     const long long pos = (p.starts ? p.starts[s] : 0) + (t - p.cu[s]);
     const int page = page_of(p.c, s, pos, slot);

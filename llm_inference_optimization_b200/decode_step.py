@@ -416,8 +416,8 @@ class DecodeModel:
 
         ``tokens [T]`` int64, sequence b's new ones at ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``); each attends to its sequence
         up to itself.  Returns logits ``[T, vocab]`` and advances ``seq_lens`` by the counts (a caller that rejects drafted
-        tokens subtracts them again).  Tokens behind ``cu_new[B]`` are padding: nothing is stored for them and their logits mean
-        nothing.  The cache must have room for the new tokens (``init_cache(extra_tokens=)``), as for :meth:`step`.  Models with
+        tokens subtracts them again).  Tokens before ``cu_new[0]`` and from ``cu_new[B]`` on are padding: nothing is stored for them and their
+        logits mean nothing.  The cache must have room for the new tokens (``init_cache(extra_tokens=)``), as for :meth:`step`.  Models with
         4-bit keys and values on a GPU."""
         if not (self.fused_glue and self.k_bits == 4):
             raise RuntimeError("extend needs the CUDA glue path and a cache of 4-bit keys and values (k_bits=4, v_bits=4)")

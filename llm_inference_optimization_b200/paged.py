@@ -336,7 +336,8 @@ def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, 
     positions ``kv.seq_lens[b]``, ``+ 1``, ...; ``seq_lens`` is read, not advanced.  ``rope`` (a ``RotaryEmbedding``;
     ``None``: no rotation) turns q and k at those positions, or at ``positions`` (int32 or int64 ``[T]``) where the place in
     the cache is not the place in the text (an evicted, compacted cache).  Returns the rotated query ``[T, Hq, D]``: fp16, or
-    ``q_out`` (fp16 or bf16).  Rows behind ``cu_new[B]`` are left alone.  Tokens past a sequence's page list are not stored;
+    ``q_out`` (fp16 or bf16).  Rows before ``cu_new[0]`` and from ``cu_new[B]`` on belong to no sequence (part of a batch, padding)
+    and are left alone.  Tokens past a sequence's page list are not stored;
     neither is one whose page-table entry lies outside the pool, which sets ``SKV_DEV_BAD_PAGE`` (2) in ``status`` (an
     int32 device tensor of one element).  Serves ``PagedKV4`` (D 64 or 128) and every ``PagedKV`` (D 128); a rotary width
     must be a multiple of 16 (interleaved: of 8).  Block metadata is not kept current: rebuild it (``build_block_meta``).
@@ -382,7 +383,7 @@ def read_tokens(kv: "PagedKV | PagedKV4", cu: Tensor, rows: int, *, starts: Tens
 
     Rows ``cu[b]..cu[b+1]`` (int32 ``[B+1]``, ``cu[B] <= rows``) are positions ``starts[b]``, ``+ 1``, ... (int32 ``[B]``;
     ``None``: from 0) of sequence b: the prefix that a chunk of prompt attends to through another kernel, or a check of what
-    was stored.  ``kv.seq_lens`` is not consulted.  Rows behind ``cu[B]`` are not written; a position without a page reads as
+    was stored.  ``kv.seq_lens`` is not consulted.  Rows before ``cu[0]`` and from ``cu[B]`` on are not written; a position without a page reads as
     zeros (``status`` as in :func:`append_tokens`)."""
     pools, layout, table, Hkv, D, dev = _token_cache(kv)
     _C._require((dtype is torch.float16 or dtype is torch.bfloat16) and rows >= 0, "read_tokens returns fp16 or bf16 rows")

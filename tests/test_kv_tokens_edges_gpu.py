@@ -1,0 +1,96 @@
+"""Append, read-back and attention where a batch's offsets are unusual: offsets that begin above zero (part of a batch), offsets
+that do not ascend; every buffer lies between bytes that must stay as they are."""
+import pytest
+import torch
+
+from kv4_oracle import ints, offsets, page_table
+from llm_inference_optimization_b200 import _lib, _workspace, paged
+from test_kv_tokens_gpu import FORMATS, empty_cache
+
+pytestmark = pytest.mark.gpu
+MARK = 0xA5
+
+
+def guarded(shape, dtype, dev, raws):
+    """A tensor of MARK bytes with 4096 more of them on either side."""
+    n = int(torch.tensor(shape).prod()) * torch.empty((), dtype=dtype).element_size()
+    raw = torch.full((n + 8192,), MARK, dtype=torch.uint8, device=dev)
+    raws.append(raw)
+    return raw[4096:4096 + n].view(dtype).view(shape)
+
+
+def untouched(raws):
+    return all(bool((r[:4096] == MARK).all() and (r[-4096:] == MARK).all()) for r in raws)
+
+
+def read_into(kv, cu, starts, K, V):
+    """``paged.read_tokens`` into given buffers, so that rows which are not written can be told."""
+    pools, layout, table, Hkv, D, dev = paged._token_cache(kv)
+    rc = _lib.load().skv_read_tokens(*pools, table, cu.data_ptr(), starts.data_ptr(), K.data_ptr(), V.data_ptr(), 0, K.shape[0], kv.batch,
+                                     Hkv, D, *layout, None, dev.index, _workspace.stream(dev.index))
+    _lib.check(rc, "read_tokens")
+
+
+def cache_bytes(kv):
+    return [t.view(torch.uint8) for t in ((kv.buf,) if isinstance(kv, paged.PagedKV4) else (kv.k_pool, kv.v_pool, kv.k_scale, kv.v_scale))]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("B,first", [(2, 3), (300, 5)])      # counted by all lanes of a row; searched
+def test_rows_before_the_first_offset_belong_to_nobody(cuda_device, fmt, B, first):
+    """Part of a batch: its offsets begin above zero, and the rows before them change no cached token, no query row, no row read."""
+    Hq, Hkv, D = 2, 2, 128
+    g = torch.Generator().manual_seed(B)
+    old, new = [100 + i % 7 for i in range(B)], [2 + i % 3 for i in range(B)]
+    size = 48 if fmt == "pools" else 16
+    table, total = page_table([(a + n + size - 1) // size for a, n in zip(old, new)], 0, g)
+    part, whole = (empty_cache(fmt, total, Hkv, D, table, ints(*old), B, cuda_device) for _ in range(2))
+    T = first + sum(new)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).half().to(cuda_device)
+    cu = (offsets(new) + first).to(cuda_device)
+    raws = []
+    q = paged.append_tokens(qkv, part, Hq, cu_new=cu, q_out=guarded((T, Hq, D), torch.float16, cuda_device, raws))
+    want = paged.append_tokens(qkv[first:], whole, Hq, cu_new=cu - first)
+    assert torch.equal(q[first:], want) and (q[:first].view(torch.uint8) == MARK).all()
+    assert all(torch.equal(a, b) for a, b in zip(cache_bytes(part), cache_bytes(whole)))
+    K, V = (guarded((T, Hkv, D), torch.float16, cuda_device, raws) for _ in range(2))
+    read_into(part, cu, part.seq_lens, K, V)
+    for got, rows in zip((K, V), paged.read_tokens(whole, cu - first, T - first, starts=whole.seq_lens)):
+        assert torch.equal(got[first:], rows) and (got[:first].view(torch.uint8) == MARK).all()
+    assert untouched(raws)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cu", [(5, 2, 9, 1), (-7, 100, -100, 3), (2 ** 31 - 1, -2 ** 31, 0, 9), (9, 9, 9, 0)])
+def test_offsets_that_do_not_ascend_write_nothing_else(cuda_device, D, cu):
+    """Whatever sequence a row is given, it lands in a page of the table: pages that no sequence owns and the bytes around every
+    buffer stay."""
+    raws = []
+    table, total = page_table([3, 3, 3], 4, torch.Generator().manual_seed(4))
+    buf = guarded((total, 2, 18, D), torch.uint8, cuda_device, raws)
+    kv = paged.PagedKV4(buf, table.to(cuda_device), ints(0, 0, 0).to(cuda_device), 3)
+    qkv = torch.randn(9, 6 * D, generator=torch.Generator().manual_seed(3)).half().to(cuda_device)
+    at = ints(*cu).to(cuda_device)
+    half = lambda *s: guarded(s, torch.float16, cuda_device, raws)  # noqa: E731
+    paged.append_tokens(qkv, kv, 2, cu_new=at, q_out=half(9, 2, D))
+    read_into(kv, at, kv.seq_lens, half(9, 2, D), half(9, 2, D))
+    kv.decode(torch.randn(9, 2, D, device=cuda_device).half(), 0.125, cu_q=at, out=half(9, 2, D))
+    torch.cuda.synchronize()
+    assert untouched(raws)
+    unowned = sorted(set(range(total)) - set(table.flatten().tolist()))
+    assert len(unowned) == 4 and (buf[unowned] == MARK).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_part_of_a_batch(cuda_device, D):
+    raws, g = [], torch.Generator().manual_seed(D)
+    table, total = page_table([20, 3], 0, g)
+    kv = empty_cache("kv4", total, 2, D, table, ints(0, 0), 2, cuda_device)
+    new = [300, 40]
+    paged.append_tokens(torch.randn(340, 4 * D, generator=g).half().to(cuda_device), kv, 0, cu_new=offsets(new).to(cuda_device))
+    kv.seq_lens += ints(*new).to(cuda_device)
+    q = torch.randn(12, 8, D, generator=g).half().to(cuda_device)
+    cu = ints(3, 7, 9).to(cuda_device)
+    out = kv.decode(q, D ** -0.5, cu_q=cu, out=guarded((12, 8, D), torch.float16, cuda_device, raws))
+    assert torch.equal(out[3:9], kv.decode(torch.roll(q, -3, 0), D ** -0.5, cu_q=cu - 3)[:6])   # as many rows: the same split of the work
+    assert (out[:3].view(torch.uint8) == MARK).all() and (out[9:].view(torch.uint8) == MARK).all() and untouched(raws)
