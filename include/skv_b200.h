@@ -231,7 +231,10 @@ int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype
  *   sequence and are left alone, in q_out too.
  *   seq_lens is not modified.  A position past max_pages * page_size stores nothing, nor does one whose page-table entry
  *   lies outside [0, num_pages), which sets SKV_DEV_BAD_PAGE in *status (optional).  A row (4-bit: a group of 32
- *   channels) that is not finite is stored with scale NaN.  rotary_dim is a multiple of 16 (interleaved: of 8).
+ *   channels) that is not finite is stored with scale NaN.  Scales are amax * fp32(1 / top code) in every format (top codes 7,
+ *   127, 448; bf16 in 4-bit records), 1 for a row of zeros (4-bit records: 0).  rotary_dim is a multiple of 16 (interleaved: of 8).
+ *   (skv_rope_quant_append divides, amax / top code, and works angles out in 32 bits: scales may differ from its in the last bit,
+ *   and far positions by what 32 bits lose of their angle.  One sequence is best filled by one of the two.)
  * skv_read_tokens: row t with cu[b] <= t < cu[b + 1] receives the token at position starts[b] + t - cu[b] (starts NULL: 0)
  *   of sequence b as values, k_out / v_out [T, Hkv, D] fp16 (bf16 with out_is_bf16), code * scale rounded once; zeros where
  *   the cache has no page.  Rows before cu[0] and from cu[B] on are left alone.
@@ -253,7 +256,7 @@ int skv_read_tokens(const void* k_pool, const void* v_pool, const float* k_scale
 
 /* ---- dense GQA decode over a paged cache held in 4 bits -----------------------------
  * No reference counterpart.  Keys and values in page records of 16 tokens, 18 * D bytes per (page, head): 8 D bytes of key
- * codes, 8 D of value codes, 2 D of scales.  Every 32 channels of a row share a bf16 scale = bf16(amax / 7) (0 for zeros,
+ * codes, 8 D of value codes, 2 D of scales.  Every 32 channels of a row share a bf16 scale = bf16(amax * fp32(1 / 7)) (0 for zeros,
  * NaN for a group that is not finite), code = clamp(rne(x / scale), -7, 7) in the nibble code + 8, even nibble low.  Token
  * t = 4i + 2j + e of a page has place 8j + 2i + e:
  *   keys    byte place * D/2 + c * D/8 + 4w + n/2                    channel 32w + 8c + n  (c < 4, n < 8)

@@ -110,7 +110,10 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
 }
 
 // Eight fp32 channels of a row, quantised with one scale for LANES lanes: LANES = 4 groups of 32 (bf16 scale, 4-bit
-// records), LPR: whole rows (fp32 scale, qmax).
+// records), LPR: whole rows (fp32 scale).  One rule makes the scale in every format: amax times the fp32 number nearest to
+// 1 / top code (7, 127, 448).  That is what torch makes of amax / 7 on the GPU, so rows quantised there and here hold the same
+// codes; many values lie exactly between two codes, and which one they take follows the last bit of the scale.
+// (skv_rope_quant_append divides: a scale may differ from its in the last bit, and codes of values between two then.)
 template <int LANES>
 __device__ __forceinline__ uint32_t abs_max_bits(const float (&x)[8], unsigned group) {
     uint32_t m = 0;   // the bits of |x| order like |x|, infinities and NaN on top
@@ -142,7 +145,7 @@ __device__ __forceinline__ void store_kv4(const float (&x)[8], uint8_t* rec, int
     constexpr int W = D / 32;
     const uint32_t m = abs_max_bits<4>(x, group);
     const bool finite = m < 0x7f800000u;
-    const uint16_t sb = finite ? __bfloat16_as_ushort(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), 7.f))) : (uint16_t)0x7fc0;
+    const uint16_t sb = finite ? __bfloat16_as_ushort(__float2bfloat16_rn(__fmul_rn(__uint_as_float(m), 1.f / 7.f))) : (uint16_t)0x7fc0;
     const float s = bf16_bits_to_f(sb);
     // (a scale of zero or NaN: all codes zero.  Scales below the normal range hold no more than that either.)
     const uint32_t word = finite && s >= 1.1754944e-38f ? nibbles8(x, s, __frcp_rn(s)) : 0x88888888u;
@@ -167,16 +170,14 @@ __device__ __forceinline__ void store_kv4(const float (&x)[8], uint8_t* rec, int
     if (live && c == 0) *reinterpret_cast<uint16_t*>(rec + kv4_scales<D>(slot) + (IS_V ? D / 16 : 0) + 2 * w) = sb;
 }
 
-// Rows with one fp32 scale: amax / qmax, 1 for a zero row, NaN for a row that is not finite.  BITS4: nibbles, else bytes.
+// Rows with one fp32 scale: 1 for a zero row, NaN for a row that is not finite.  BITS4: nibbles, else bytes.
 template <int LPR, int CACHE, bool BITS4>
 __device__ __forceinline__ void store_row(const float (&x)[8], uint8_t* row, float* scale, int l, unsigned group, bool live) {
     constexpr bool E4M3 = !BITS4 && (CACHE == CACHE_E4M3 || CACHE == CACHE_E4M3_V4);
     const uint32_t m = abs_max_bits<LPR>(x, group);
     const bool finite = m < 0x7f800000u;
     const float amax = __uint_as_float(m);
-    // 4-bit values: amax times the number nearest 1/7, which is what torch makes of amax / 7 on the GPU (decode_step's quantiser):
-    // with 15 codes many values lie exactly between two of them, and which one they take follows the last bit of the scale
-    const float top = BITS4 ? __fmul_rn(amax, 1.f / 7.f) : __fdiv_rn(amax, E4M3 ? 448.f : 127.f);
+    const float top = __fmul_rn(amax, 1.f / (BITS4 ? 7.f : E4M3 ? 448.f : 127.f));
     const float s = finite ? (amax > 0.f ? top : 1.f) : __uint_as_float(0x7fc00000u);
     const float r = __frcp_rn(s);
     const bool any = finite && s >= 1.1754944e-38f;  // (a scale that is NaN, or below the normal range: all codes zero)

@@ -1,9 +1,10 @@
 // The 4-bit page record, shared by the kernels that write, read and attend to it, and the rotary angle.
 //
 // A record holds 16 tokens of one kv-head in 18 * D bytes: 8 D of key codes, 8 D of value codes, 2 D of scales.  Every
-// 32 channels of a row share one bf16 scale = bf16(amax / 7) (bf16: as wide a range as fp32, so no row over- or
+// 32 channels of a row share one bf16 scale = bf16(amax * fp32(1 / 7)) (bf16: as wide a range as fp32, so no row over- or
 // underflows it; the codes are made with the ROUNDED scale, so its 8 bits cost nothing but a sliver of the code range);
-// code = clamp(rne(x / scale), -7, 7), stored as the nibble code + 8, even nibble low.  An all-zero group has scale 0;
+// code = clamp(rne(x / scale), -7, 7), stored as the nibble code + 8, even nibble low.  An all-zero group has scale 0
+// (and one whose scale is below fp32's normal range all codes 0);
 // a group that holds a NaN or an infinity has scale NaN, so that whoever attends to it gets NaN and not a plausible number.
 //
 // The order inside a record is that of the attention kernel's matrix fragments, so that its lanes fetch their operands

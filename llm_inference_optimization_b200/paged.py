@@ -197,7 +197,8 @@ def rope_quant_append(qkv: Tensor, kv: PagedKV, Hq: int, rope_theta: float, *, m
     ``[B, Hq, 128]`` fp16.  ``kv.seq_lens`` is read, not advanced.  With ``meta`` (the tensor
     ``build_block_meta`` returns) the min/max metadata of the block that receives the token is updated in the
     same launch (``skv_rope_quant_append``).  A page-table entry outside the pool stores nothing and sets bit
-    ``SKV_DEV_BAD_PAGE`` (2) in ``status`` (an int32 device tensor of one element), when one is given.
+    ``SKV_DEV_BAD_PAGE`` (2) in ``status`` (an int32 device tensor of one element), when one is given.  Angles are worked out
+    in 32 bits (off by some 6e-8 of themselves: 0.006 radians at position 100000); :func:`append_tokens` works them out in 64.
     """
     strides = _pool_args(kv)
     _, Hkv, P, D = kv.k_pool.shape
@@ -341,6 +342,9 @@ def append_tokens(qkv: Tensor, kv: "PagedKV | PagedKV4", Hq: int, rope=None, *, 
     neither is one whose page-table entry lies outside the pool, which sets ``SKV_DEV_BAD_PAGE`` (2) in ``status`` (an
     int32 device tensor of one element).  Serves ``PagedKV4`` (D 64 or 128) and every ``PagedKV`` (D 128); a rotary width
     must be a multiple of 16 (interleaved: of 8).  Block metadata is not kept current: rebuild it (``build_block_meta``).
+    Scales are ``amax * fp32(1 / top code)`` in every format, as torch divides by a number on the GPU; ``rope_quant_append`` divides
+    and has 32-bit angles, so the two may differ in a scale's last bit and, at far positions, in the angle: fill a sequence by
+    one of them.
     """
     pools, layout, table, Hkv, D, dev = _token_cache(kv)
     bf16 = qkv.dtype is torch.bfloat16

@@ -5,6 +5,7 @@ import torch
 
 from kv4_oracle import ints, offsets, page_table
 from llm_inference_optimization_b200 import _lib, _workspace, paged
+from llm_inference_optimization_b200 import decode_step as ds
 from test_kv_tokens_gpu import FORMATS, empty_cache
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,37 @@ def test_attention_of_part_of_a_batch(cuda_device, D):
     out = kv.decode(q, D ** -0.5, cu_q=cu, out=guarded((12, 8, D), torch.float16, cuda_device, raws))
     assert torch.equal(out[3:9], kv.decode(torch.roll(q, -3, 0), D ** -0.5, cu_q=cu - 3)[:6])   # as many rows: the same split of the work
     assert (out[:3].view(torch.uint8) == MARK).all() and (out[9:].view(torch.uint8) == MARK).all() and untouched(raws)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_take_the_codes_of_torchs_quantisers(cuda_device, fmt, dtype):
+    """Scales and codes of unrotated rows are those that torch makes on the GPU, values between two codes among them.  E4M3 codes are
+    compared as numbers: the kernel's division by correction makes +0 of -0 (fma(-q, s, x) is +0 there), the same value."""
+    Hkv, D, T = 2, 128, 700
+    table, total = page_table([15 if fmt == "pools" else 44], 0, torch.Generator().manual_seed(1))
+    kv = empty_cache(fmt, total, Hkv, D, table, ints(0), 1, cuda_device)
+    x = torch.randn(T, 2 * Hkv, D, generator=torch.Generator().manual_seed(2)) * torch.exp2(torch.arange(T) % 13 - 6.0)[:, None, None]
+    x[::3] = (x[::3] * 4).round() / 4                # a coarse grid: many values lie between two codes
+    x = x.to(dtype).to(cuda_device)
+    paged.append_tokens(x.flatten(1), kv, 0, cu_new=offsets([T]).to(cuda_device))
+    t = torch.arange(T, device=cuda_device)
+    size = 48 if fmt == "pools" else 16
+    page, slot = kv.page_table[0, t // size].long(), t % size
+    held = lambda p: p.transpose(1, 2)[page, slot]  # noqa: E731
+    for rows, which in ((x[:, :Hkv], "k"), (x[:, Hkv:], "v")):
+        if fmt == "kv4":
+            codes, scale = ds.quantize_groups_int4(rows)
+            parts = paged.unpack_kv4(kv.buf)[:2] if which == "k" else paged.unpack_kv4(kv.buf)[2:]
+        else:
+            parts = (kv.k_pool, kv.k_scale) if which == "k" else (kv.v_pool, kv.v_scale)
+            if fmt == "mixed" and which == "v":
+                codes, scale = ds.quantize_rows_int4(rows)
+            elif fmt in ("mixed", "e4m3"):
+                codes, scale = ds.quantize_rows_e4m3(rows)
+                codes, parts = codes.float(), (parts[0].float(), parts[1])
+            else:
+                amax = rows.float().abs().amax(-1)
+                scale = torch.where(amax > 0, amax / 127.0, torch.ones_like(amax))
+                codes = (rows.float() / scale[..., None]).round().to(torch.int8)
+        assert torch.equal(held(parts[1]), scale) and torch.equal(held(parts[0]), codes)
