@@ -117,21 +117,26 @@ class LayerCache:
         """Quantise the new token's ``k, v [B, n_kv, D]`` and store them at position ``seq_lens[b]``."""
         B = k.shape[0]
         lens = seq_lens.long()
-        page = page_table[torch.arange(B, device=k.device), lens // 16].long()
+        room, pages = page_table.shape[1], self.buf.shape[0]
+        page = page_table[torch.arange(B, device=k.device), (lens // 16).clamp(max=room - 1)].long()
         slot = lens % 16
+        # A sequence that has outgrown its pages stores nothing: its row becomes a copy of one that has a page (the same values
+        # written twice), or, where none has, of what page 0 holds already.  No index leaves the pool and nothing waits for the host.
+        ok = (lens // 16 < room) & (page >= 0) & (page < pages)
+        row = torch.where(ok, torch.arange(B, device=k.device), ok.int().argmax())
+        page, slot, k, v, some = page[row].clamp_(0, pages - 1), slot[row], k[row], v[row], ok.any()
         if self.k_bits == 4:
             parts = paged.unpack_kv4(self.buf[page])       # the B pages that receive a token, taken apart and put back
             b = torch.arange(B, device=k.device)
             for part, new in zip(parts, (*quantize_groups_int4(k), *quantize_groups_int4(v))):
-                part[b, :, slot] = new
+                part[b, :, slot] = torch.where(some, new, part[b, :, slot])
             self.buf[page] = paged.pack_kv4(*parts)
             return
         kc, ksc = quantize_rows_e4m3(k)
         vc, vsc = quantize_rows_int4(v) if self.v_bits == 4 else quantize_rows_e4m3(v)
-        self.k.view(torch.uint8)[page, :, slot] = kc.view(torch.uint8)
-        self.v.view(torch.uint8)[page, :, slot] = vc.view(torch.uint8)
-        self.ks[page, :, slot] = ksc
-        self.vs[page, :, slot] = vsc
+        for pool, new in ((self.k.view(torch.uint8), kc.view(torch.uint8)), (self.v.view(torch.uint8), vc.view(torch.uint8)),
+                          (self.ks, ksc), (self.vs, vsc)):
+            pool[page, :, slot] = torch.where(some, new, pool[page, :, slot])
 
 
 AttentionFn = Callable[[Tensor, LayerCache, Tensor, Tensor, float, int], Tensor]
@@ -216,6 +221,8 @@ class DecodeModel:
         self.caches: list[LayerCache] = []
         self.page_table: Tensor | None = None
         self.seq_lens: Tensor | None = None
+        self.room: Tensor | None = None        # int32 [B]: tokens that each sequence's own pages hold
+        self.status: Tensor | None = None      # int32 [1]: set by a kernel that met a page-table entry outside the pool (check_cache)
         self.max_seq_len = 0
 
     # ------------------------------------------------------------------ per-layer sparsity schedule
@@ -263,7 +270,8 @@ class DecodeModel:
         No prefill pass is run (only the decode step is the workload): ``fill="normal"`` writes N(0,1)
         keys/values quantised row by row to FP8; ``fill="random_codes"`` writes uniformly random FP8 codes with
         scales near 0.008 (values within about +-4), which is much faster to generate for a 70 GB cache and
-        costs the kernels the same time.  Pages are assigned to (sequence, logical page) by a seeded permutation.
+        costs the kernels the same time.  Pages are assigned to (sequence, logical page) by a seeded permutation; every
+        sequence has pages for its length and ``extra_tokens`` more, and the table's entries behind them name no page (-1).
         """
         cfg, dev = self.cfg, self.device
         B = seq_lens.numel()
@@ -272,13 +280,15 @@ class DecodeModel:
         total = sum(pages_per_seq)
         g = torch.Generator().manual_seed(seed)
         perm = torch.randperm(total, generator=g)
-        table = torch.zeros((B, cap), dtype=torch.int32)
+        table = torch.full((B, cap), -1, dtype=torch.int32)
         o = 0
         for b, n in enumerate(pages_per_seq):
             table[b, :n] = perm[o:o + n].to(torch.int32)
             o += n
         self.page_table = table.to(dev)
         self.seq_lens = seq_lens.to(device=dev, dtype=torch.int32).clone()
+        self.room = torch.tensor([16 * n for n in pages_per_seq], dtype=torch.int32, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.max_seq_len = cap * 16
         self.caches = []
         gd = torch.Generator(device=dev)
@@ -312,6 +322,18 @@ class DecodeModel:
             self.caches.append(c)
         self.metas = [None] * cfg.layers
         self._build_missing_metas()
+
+    def check_cache(self) -> None:
+        """Raise if a sequence has outgrown its own pages (or a kernel met a page-table entry outside the pool).
+
+        Steps and prompts never ask the host how long a sequence is: a token without a page is not stored, the others are
+        untouched, and the sequence's logits mean nothing from there on.  This waits for the device; call it between steps."""
+        over = (self.seq_lens > self.room).nonzero().flatten().tolist()
+        bad = int(self.status)
+        self.status.zero_()
+        if over or bad:
+            raise RuntimeError(f"tokens without a page were not stored: sequences {over} are longer than their pages hold "
+                               f"(init_cache(extra_tokens=)), status word {bad}")
 
     # ------------------------------------------------------------------ the step
     def _all_reduce(self, x: Tensor) -> Tensor:
@@ -370,14 +392,14 @@ class DecodeModel:
         sparse = self.layer_modes[li] == "quest"
         a = torch.empty((B, sh.n_q, D), dtype=dtype, device=qkv.device)
         if self.rope is not None:
-            q = paged.append_tokens(qkv, self._layer_kv(cache, pos), sh.n_q, self.rope, cu_new=cu)
+            q = paged.append_tokens(qkv, self._layer_kv(cache, pos), sh.n_q, self.rope, cu_new=cu, status=self.status)
             if cache.k_bits == 4:
-                return self._layer_kv(cache, new_lens).decode(q, scale, cu_q=cu, max_seq_len=self.max_seq_len, out=a)
+                return self._layer_kv(cache, new_lens).decode(q, scale, cu_q=cu, max_seq_len=self.max_seq_len, out=a, status=self.status)
             _C.fused_gqa_paged(q, cache.k, cache.v, cache.ks, cache.vs, self.page_table, new_lens, scale,
                                max_seq_len=self.max_seq_len, out=a, v_bits=cache.v_bits, after_append=self.overlap_append)
             return a
         q = paged.rope_quant_append(qkv, self._layer_kv(cache, pos), sh.n_q, self.cfg.rope_theta,
-                                    meta=self.metas[li] if sparse else None, block_size=self.quest_block)
+                                    meta=self.metas[li] if sparse else None, block_size=self.quest_block, status=self.status)
         if sparse:
             return self._quest_attention(q, li, new_lens, scale, meta_is_current=True).to(dtype)
         # the append kernel above is the launch right before this one and wrote only q and position new_lens - 1
@@ -417,8 +439,8 @@ class DecodeModel:
         ``tokens [T]`` int64, sequence b's new ones at ``cu_new[b]..cu_new[b+1]`` (int32 ``[B+1]``); each attends to its sequence
         up to itself.  Returns logits ``[T, vocab]`` and advances ``seq_lens`` by the counts (a caller that rejects drafted
         tokens subtracts them again).  Tokens before ``cu_new[0]`` and from ``cu_new[B]`` on are padding: nothing is stored for them and their
-        logits mean nothing.  The cache must have room for the new tokens (``init_cache(extra_tokens=)``), as for :meth:`step`.  Models with
-        4-bit keys and values on a GPU."""
+        logits mean nothing.  The cache must have room for the new tokens (``init_cache(extra_tokens=)``), as for :meth:`step`: those
+        without a page are not stored, which :meth:`check_cache` reports.  Models with 4-bit keys and values on a GPU."""
         if not (self.fused_glue and self.k_bits == 4):
             raise RuntimeError("extend needs the CUDA glue path and a cache of 4-bit keys and values (k_bits=4, v_bits=4)")
         if tokens.shape[0] == 0:
