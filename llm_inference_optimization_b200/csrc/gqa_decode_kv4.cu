@@ -15,10 +15,11 @@
 //     codes.  The factor 16 between the two kinds is put into the query (its own exponent is normalised first) and, for
 //     values, divided out of the rows of O at the end.  Codes are u - 8: the 8 is taken out of the scores by starting the
 //     accumulators at -8 ks sum(q), a small product of its own, and out of the value codes by an exact packed addition.
-//   * ks multiplies the fp32 partial scores of its group; vs is folded into the weights before they are rounded to fp16.
-//     (One rounding to 11 bits per weight.)  The reference that scores are taken against before exp2 only has to keep the
-//     weights within fp16: it follows the running maximum of scores and value scales in jumps of several powers of two, so
-//     a record costs one vote where an exact running maximum costs shuffles and a rescaling of O.
+//   * ks multiplies the fp32 partial scores of its group; vs is folded into the weights before they are rounded to fp16 (one
+//     rounding of each product of weight and scale).  vs is taken relative to a power of two of its group of 32 channels,
+//     which follows the largest scale seen there; the reference that scores are taken against before exp2 only has to keep
+//     the weights within fp16 and follows their running maximum in jumps of several powers of two.  So a record costs one vote
+//     where exact running maxima cost shuffles and a rescaling of O.
 //   * Tokens on the M side of both products (S^T = K Q^T, O^T = V^T P^T), up to 8 NT columns (query token, head) on the
 //     N side; P goes from the one layout to the other by movmatrix.
 //
@@ -42,9 +43,16 @@
 namespace skv {
 namespace kv4 {
 
-// Weights are kept below 2^WEIGHT_MAX (fp16 holds 2^15.99) and are at most 2^WEIGHT_AIM when their reference has just moved:
-// four powers of two before it moves again, and eleven bits for every weight down to 2^-24 of the largest.
+// Weights are kept below 2^WEIGHT_MAX and are at most 2^WEIGHT_AIM when their reference has just moved: four powers of two
+// before it moves again.  Value scales relative to their group's power of two lie below 2 (below 3.99 for bf16's topmost
+// exponent), so products stay below fp16's 65504; when the power has just moved, below 2^(1 - SCALE_ROOM): the next larger
+// scales find room (0, 1, 2: 70.1, 68.7, 68.5 us for 4 sequences of 65536 tokens, 67.9 with one power for all groups and
+// weights together).  A product has eleven bits down to 2^-22 of the largest weight times the largest scale of the same group
+// that the warp has seen, and is off by at most 2^-33 of that below (2^-25, half of fp16's smallest step, against 2^(10 - 2)).
 constexpr float WEIGHT_MAX = 14.f, WEIGHT_AIM = 10.f;
+constexpr int SCALE_ROOM = 2;
+// Sums leave the registers times 2^SUMS_DOWN: 2^14 * 2^16 tokens * 8 * the largest bf16 number times 2^-40 is within fp32.
+constexpr int SUMS_DOWN = -40;
 constexpr float NOTHING = -1e30f;     // reference of a column that has seen no token
 constexpr int MIN_UNITS = 16;         // records per CTA at least: shorter runs are all start and end
 constexpr size_t TICKET_OFF = 256, PARTIAL_OFF = 8192;
@@ -161,6 +169,23 @@ template <int N> __device__ __forceinline__ float group_scale(const uint32_t (&s
     return (w & 1) ? bf_hi(s[first + (w >> 1)]) : bf_lo(s[first + (w >> 1)]);
 }
 template <bool V> struct Constant { static constexpr bool value = V; };
+
+// The power of two that a group's value scales are multiplied by, a bf16 number of field 254 - e for scales of fields up to e
+// (fields with the bias 127, e = 0 .. 253: 2^-127 is no normal number, so the topmost field counts as the one below it).
+constexpr uint32_t DOWN_NONE = 254u << 7;             // no scale yet, or numbers below the normal range: 2^127
+template <int N> __device__ __forceinline__ int exponent_of(const uint32_t (&down)[N], int w) {
+    return 254 - (int)(down[w >> 1] >> ((w & 1) * 16 + 7) & 0xffu);
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ constexpr float exp2_of(int e) {
+    float x = 1.f;
+    for (int i = 0; i < (e < 0 ? -e : e); ++i) x *= e < 0 ? 0.5f : 2.f;
+    return x;
+}
 
 // Column `col` of the item's list (query token col / G, head col % G), channels d .. d + 3
 __device__ __forceinline__ void store_out(const Params& p, const Segment& x, int D, int col, int d, float4 v, float L) {
@@ -520,8 +545,9 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
             ref[nt][0] = ref[nt][1] = NOTHING;
             lrun[nt][0] = lrun[nt][1] = 0.f;
         }
-        uint32_t vref = 0;                             // bf16 bits, twice: no value scale of this warp so far is larger
-        float room = WEIGHT_MAX + 60.f;                // largest s - ref that keeps a weight below 2^WEIGHT_MAX: that less log2 vref
+        uint32_t vdown[W / 2];                         // the groups' powers of two, two a word: no scale of this warp so far reaches 2 times it
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) vdown[i] = DOWN_NONE | DOWN_NONE << 16;
 
         const int tok_a = 4 * (g >> 1) + (g & 1);      // rows g and g + 8 of the score tile are tokens tok_a and tok_a + 2
         int out_off = 0;                               // ring offset of the record that is worked on
@@ -575,12 +601,16 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                     if (t0 + 2 >= end_tok) vb_scale[i] = 0u;
                 }
             }
-            // Weights are exp2(s - ref) * vs, ref any number that keeps them in fp16's range: it moves only when a score or a
-            // value scale leaves the room there is, which is seldom after the first record.
-            uint32_t vtop = vref;
+            // Weights are exp2(s - ref), ref any number that keeps them in fp16's range, value scales are taken relative to their
+            // group's power of two: both move only when a score or a scale leaves the room there is, seldom after the first record.
+            uint32_t large = 0u;                       // bit 14 of a bf16 number: 2 and more
             float t[NT][4], top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < W / 2; ++i) vtop = __vmaxu2(vtop, __vmaxu2(va_scale[i], vb_scale[i]));
+            for (int i = 0; i < W / 2; ++i) {
+                va_scale[i] = mul_bf16x2(va_scale[i], vdown[i]);
+                vb_scale[i] = mul_bf16x2(vb_scale[i], vdown[i]);
+                large |= va_scale[i] | vb_scale[i];
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -589,19 +619,37 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                     if (MASKED && hidden(j, nt)) t[nt][j] = -INFINITY;
                     top = fmaxf(top, t[nt][j]);
                 }
-            if (__any_sync(0xffffffffu, top > room || vtop != vref)) {
-                // bound of every value scale so far: its exponent's largest number; the exponent is clamped to what keeps
-                // sums of weights in fp32's range (beyond it weights lose bits, far below 2^-60)
-                uint32_t v = vref & 0xffffu;           // (a scale that is NaN is for those who see it, not for the bound)
+            if (__any_sync(0xffffffffu, top > WEIGHT_MAX || (large & 0x40004000u) != 0u)) {
+                // the largest exponent of each group's value scales so far (a scale that is NaN or infinite is for those who see
+                // it, not for the bound); the scales themselves are fetched once more
+                uint32_t ra[W], rb[W];
+                lds<D / 8>(rec + 16 * D + g * (D / 8), ra);
+                lds<D / 8>(rec + 17 * D + g * (D / 8), rb);
 #pragma unroll
-                for (int i = 0; i < W / 2; ++i)
+                for (int w = 0; w < W; ++w) {
+                    const int half = (w & 1) * 16, old = exponent_of(vdown, w);
+                    const uint32_t xa = MASKED && t0 >= end_tok ? 0u : ra[W / 2 + (w >> 1)] >> half & 0xffffu;
+                    const uint32_t xb = MASKED && t0 + 2 >= end_tok ? 0u : rb[W / 2 + (w >> 1)] >> half & 0xffffu;
+                    int e = old;
+                    if (xa < 0x7f80u) e = max(e, (int)(xa >> 7));
+                    if (xb < 0x7f80u) e = max(e, (int)(xb >> 7));
+                    e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e);
+                    if (e > old && old < 253) {        // (the same for all lanes)
+                        // O of the group moves to the new power of two, exactly while it does not underflow
+                        e = min(e + SCALE_ROOM, 253);
+                        const float c = e - old < 127 ? __uint_as_float((uint32_t)(127 - e + old) << 23) : 0.f;
+                        vdown[w >> 1] = (vdown[w >> 1] & (0xffff0000u >> half)) | (uint32_t)(254 - e) << (7 + half);
 #pragma unroll
-                    for (uint32_t x : {va_scale[i] & 0xffffu, va_scale[i] >> 16, vb_scale[i] & 0xffffu, vb_scale[i] >> 16})
-                        if (x < 0x7f80u) v = max(v, x | 0x7fu);
-                v = __reduce_max_sync(0xffffffffu, v);
-                vref = v | (v << 16);
-                const float e = fminf(fmaxf((float)((int)(v >> 7 & 0xffu) - 126), -60.f), 100.f);
-                room = WEIGHT_MAX - e;
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) { o[nt][2 * w][j] *= c; o[nt][2 * w + 1][j] *= c; }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) {
+                    va_scale[i] = mul_bf16x2(MASKED && t0 >= end_tok ? 0u : ra[W / 2 + i], vdown[i]);
+                    vb_scale[i] = mul_bf16x2(MASKED && t0 + 2 >= end_tok ? 0u : rb[W / 2 + i], vdown[i]);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -616,8 +664,8 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                             sx = fmaxf(sx, __shfl_xor_sync(0xffffffffu, sx, x));
                             tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
                         }
-                        if (tx > room) {               // (the same for all lanes of a column)
-                            const float moved = sx + e - WEIGHT_AIM;
+                        if (tx > WEIGHT_MAX) {         // (the same for all lanes of a column)
+                            const float moved = sx - WEIGHT_AIM;
                             const float c = fast_exp2(ref[nt][j] - moved);
                             ref[nt][j] = moved;
                             lrun[nt][j] *= c;
@@ -690,15 +738,17 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                 l += __shfl_xor_sync(0xffffffffu, l, 4);
                 l += __shfl_xor_sync(0xffffffffu, l, 8);
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
-                if (g == 0) merge_ml[warp * NC + c] = make_float2(ref[nt][j], l);
+                if (g == 0) merge_ml[warp * NC + c] = make_float2(ref[nt][j], l * exp2_of(SUMS_DOWN));
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    // rows g hold (even + 16 odd) 2^-24, rows g + 8 odd 2^-20
+                    // rows g hold (even + 16 odd) 2^-24, rows g + 8 odd 2^-20, both less the group's power of two
+                    const int e = exponent_of(vdown, w);
+                    const float up = __uint_as_float(e ? (uint32_t)e << 23 : 0x400000u);   // 2^(e - 127)
                     float4 v;
-                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * 16777216.f;
-                    v.y = o[nt][2 * w][j + 2] * 1048576.f;
-                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * 16777216.f;
-                    v.w = o[nt][2 * w + 1][j + 2] * 1048576.f;
+                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * exp2_of(24 + SUMS_DOWN) * up;
+                    v.y = o[nt][2 * w][j + 2] * exp2_of(20 + SUMS_DOWN) * up;
+                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * exp2_of(24 + SUMS_DOWN) * up;
+                    v.w = o[nt][2 * w + 1][j + 2] * exp2_of(20 + SUMS_DOWN) * up;
                     *reinterpret_cast<float4*>(merge + (warp * NC + c) * S::ROW + 32 * w + 4 * g) = v;
                 }
             }

@@ -1,0 +1,87 @@
+"""4-bit attention where value scales or values lie far apart: groups of channels of very different size in one row, a
+large token that hardly counts, values near the ends of bf16's range."""
+import pytest
+import torch
+
+from kv4_oracle import attend, close, half_step, ints, page_table, quantise4, values4
+from llm_inference_optimization_b200 import paged
+
+pytestmark = pytest.mark.gpu
+
+
+class Cache:
+    """One kv-head a sequence of the given lengths; ``k`` and ``v`` [tokens, D] of the sequences one behind the other."""
+
+    def __init__(self, k, v, lens, dev):
+        D, g = k.shape[1], torch.Generator().manual_seed(1)
+        self.lens, self.table = lens, None
+        self.table, pages = page_table([(n + 15) // 16 for n in lens], 1, g)
+        rows = [torch.zeros(pages, 1, 16, D), torch.zeros(pages, 1, 16, D)]
+        at = 0
+        for b, n in enumerate(lens):
+            t = torch.arange(n)
+            for dst, src in zip(rows, (k, v)):
+                dst[self.table[b, t // 16].long(), 0, t % 16] = src[at:at + n]
+            at += n
+        (self.kc, self.ks), (self.vc, self.vs) = (quantise4(x) for x in rows)
+        self.kv = paged.PagedKV4(paged.pack_kv4(self.kc, self.ks, self.vc, self.vs).to(dev), self.table.to(dev), ints(*lens).to(dev), len(lens))
+
+    def rows(self, b):
+        t = torch.arange(self.lens[b])
+        row = lambda x: x.transpose(1, 2)[self.table[b, t // 16].long(), t % 16]  # noqa: E731
+        return values4(row(self.kc), row(self.ks)), values4(row(self.vc), row(self.vs)), row(self.vs).double().repeat_interleave(32, -1)
+
+    def check(self, q, scale, dev, dtype):
+        """Against the 64-bit formula.  A weight times its value scale has 11 bits (in attend's bound) down to 2^-22 of the largest
+        weight times the largest scale of the value's own 32 channels, and is off by at most 2^-33 of that below (half of fp16's
+        smallest step, 2^-25, where that product is at least 2^8); codes are at most 7, with the 8 that the kernel takes out
+        of them 15."""
+        got = self.kv.decode(q.to(dev), scale, out=torch.empty(q.shape, dtype=dtype, device=dev))
+        want, tol = [], []
+        for b, n in enumerate(self.lens):
+            k, v, step = self.rows(b)
+            o, t = attend(q[b:b + 1], k, v, step, scale, 1)
+            p = torch.softmax(q[b].double() @ k[:, 0].T * scale, -1)                          # [Hq, n]
+            tiny = p.amax(-1)[:, None] * step[:, 0].amax(0) * (15 * 2.0 ** -33)                # [Hq, D], a token
+            tol.append(t + n * tiny)
+            want.append(o)
+        want, tol = torch.cat(want), torch.cat(tol)
+        close(got, want, tol + half_step(want, dtype))
+        return want
+
+
+def normal(shape, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq", [4, 12])              # 8 and 16 columns a pass
+@pytest.mark.parametrize("bits", [20, 34, 60, 100])
+def test_groups_of_very_different_size(cuda_device, D, Hq, bits):
+    """The channels of one group of 32 are 2^bits times those of another, in every row: each group keeps its own eleven bits."""
+    lens = [500, 33]
+    v = normal((533, D), 2)
+    v[:, 32:64] *= 2.0 ** (bits // 2)
+    v[:, :32] *= 2.0 ** -(bits - bits // 2)
+    Cache(normal((533, D), 1), v, lens, cuda_device).check(normal((2, Hq, D), 3).half(), D ** -0.5, cuda_device, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("at", [0, 17, 250])
+def test_a_large_token_that_hardly_counts(cuda_device, D, at):
+    """One value row 2^20 times the others whose weight is below 2^-40: what the others make is kept to the bound stated."""
+    k, v = normal((300, D), 4) * 0.1, normal((300, D), 5)
+    q = normal((1, 4, D), 6)
+    q[..., 0] = 8.0
+    k[at, 0] = -40.0                                  # score -320 * scale, the others' within a few units
+    v[at] *= 2.0 ** 20
+    Cache(k, v, [300], cuda_device).check(q.half(), 0.1, cuda_device, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [-100, -60, 90, 105, 118, 124])
+def test_values_near_the_ends_of_the_range(cuda_device, D, power):
+    """Neither weights nor sums leave their range where values come near the ends of bf16's."""
+    v = normal((2100, D), 7).clamp(-4, 4) * 2.0 ** power
+    want = Cache(normal((2100, D), 8), v, [2000, 100], cuda_device).check(normal((2, 8, D), 9).half(), D ** -0.5, cuda_device, torch.bfloat16)
+    assert want.abs().max() > 0
