@@ -51,9 +51,11 @@ namespace kv4 {
 // that the warp has seen, and is off by at most 2^-33 of that below (2^-25, half of fp16's smallest step, against 2^(10 - 2)).
 constexpr float WEIGHT_MAX = 14.f, WEIGHT_AIM = 10.f;
 constexpr int SCALE_ROOM = 2;
+constexpr float BIG_SCORE = 1048576.f;   // a step of fp32 is an eighth there
+constexpr uint32_t MOVE = 0x40004000u;   // bit 14 of a bf16 number, twice: 2 and more
 // Sums leave the registers times 2^SUMS_DOWN: 2^14 * 2^16 tokens * 8 * the largest bf16 number times 2^-40 is within fp32.
 constexpr int SUMS_DOWN = -40;
-constexpr float NOTHING = -1e30f;     // reference of a column that has seen no token
+constexpr float NOTHING = -3e38f;     // reference of a column that has seen no token, near the lowest number: scores lie above it
 constexpr int MIN_UNITS = 16;         // records per CTA at least: shorter runs are all start and end
 constexpr size_t TICKET_OFF = 256, PARTIAL_OFF = 8192;
 constexpr int MAX_GRID = 160;         // CTAs of one wave (a combine keeps this many (max, sum) pairs in a warp's registers)
@@ -549,6 +551,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) vdown[i] = DOWN_NONE | DOWN_NONE << 16;
 
+        uint32_t big = 0u;                             // MOVE: a reference of this warp is far from zero
         const int tok_a = 4 * (g >> 1) + (g & 1);      // rows g and g + 8 of the score tile are tokens tok_a and tok_a + 2
         int out_off = 0;                               // ring offset of the record that is worked on
         auto record = [&](int k, auto masked_constant) {
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
             }
             // Weights are exp2(s - ref), ref any number that keeps them in fp16's range, value scales are taken relative to their
             // group's power of two: both move only when a score or a scale leaves the room there is, seldom after the first record.
-            uint32_t large = 0u;                       // bit 14 of a bf16 number: 2 and more
+            uint32_t large = big;
             float t[NT][4], top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < W / 2; ++i) {
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                     if (MASKED && hidden(j, nt)) t[nt][j] = -INFINITY;
                     top = fmaxf(top, t[nt][j]);
                 }
-            if (__any_sync(0xffffffffu, top > WEIGHT_MAX || (large & 0x40004000u) != 0u)) {
+            if (__any_sync(0xffffffffu, top > WEIGHT_MAX || (large & MOVE) != 0u)) {
                 // the largest exponent of each group's value scales so far (a scale that is NaN or infinite is for those who see
                 // it, not for the bound); the scales themselves are fetched once more
                 uint32_t ra[W], rb[W];
@@ -654,7 +657,13 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        // the column's largest score (from the score itself: t has lost it against NOTHING)
+                        // the column's largest score (from the score itself: t has lost it against NOTHING); far from zero scores
+                        // and references are rounded alike, or t would be off by as much as a step of the score
+                        if (big) {
+#pragma unroll
+                            for (int i = j; i < 4; i += 2)
+                                if (!MASKED || !hidden(i, nt)) t[nt][i] = __fsub_rn(__fmul_rn(s[nt][i], factor[nt][j]), ref[nt][j]);
+                        }
                         float sx = -INFINITY, tx = fmaxf(t[nt][j], t[nt][j + 2]);
 #pragma unroll
                         for (int i = j; i < 4; i += 2)
@@ -665,7 +674,8 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                             tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
                         }
                         if (tx > WEIGHT_MAX) {         // (the same for all lanes of a column)
-                            const float moved = sx - WEIGHT_AIM;
+                            const float moved = __fsub_ru(sx, WEIGHT_AIM);
+                            if (fabsf(moved) >= BIG_SCORE) big = MOVE;
                             const float c = fast_exp2(ref[nt][j] - moved);
                             ref[nt][j] = moved;
                             lrun[nt][j] *= c;
@@ -673,7 +683,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                             for (int i = 0; i < 2 * W; ++i) { o[nt][i][j] *= c; o[nt][i][j + 2] *= c; }
 #pragma unroll
                             for (int i = j; i < 4; i += 2) {
-                                t[nt][i] = fmaf(s[nt][i], factor[nt][j], -moved);
+                                t[nt][i] = big ? __fsub_rn(__fmul_rn(s[nt][i], factor[nt][j]), moved) : fmaf(s[nt][i], factor[nt][j], -moved);
                                 if (MASKED && hidden(i, nt)) t[nt][i] = -INFINITY;
                             }
                         }

@@ -1,5 +1,5 @@
-"""4-bit attention where value scales or values lie far apart: groups of channels of very different size in one row, a
-large token that hardly counts, values near the ends of bf16's range."""
+"""4-bit attention where value scales, values or scores lie far apart: groups of channels of very different size in one row, a
+large token that hardly counts, values near the ends of bf16's range, scores far from zero."""
 import pytest
 import torch
 
@@ -85,3 +85,33 @@ def test_values_near_the_ends_of_the_range(cuda_device, D, power):
     v = normal((2100, D), 7).clamp(-4, 4) * 2.0 ** power
     want = Cache(normal((2100, D), 8), v, [2000, 100], cuda_device).check(normal((2, 8, D), 9).half(), D ** -0.5, cuda_device, torch.bfloat16)
     assert want.abs().max() > 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [3e3, 1e5, 1e9, 1e15, 3e15, 1e16])
+def test_equal_scores_of_any_size(cuda_device, D, size, sign):
+    """Scores from 6e8 to 1e34 of either sign are scores: the softmax over equal ones is their mean."""
+    k = torch.full((20, D), sign * size)
+    v = normal((20, D), 10)
+    q = torch.full((1, 4, D), size).bfloat16()
+    c = Cache(k, v, [20], cuda_device)
+    want = c.rows(0)[1].mean(0).expand(4, D)          # all scores are equal: D * q * k
+    got = c.kv.decode(q.to(cuda_device), 1.0)
+    close(got[0], want, c.rows(0)[1].abs().mean(0) * (2.0 ** -11 + 2.0 ** -14) + c.rows(0)[2].mean(0) * 2.0 ** -13 + half_step(want, torch.bfloat16))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e5, 1e9, 1e15])
+def test_the_largest_of_large_scores_takes_all(cuda_device, D, size):
+    """Scores of 1e11 and more that are apart by a seventh of themselves: the value of the largest comes out, wherever it lies."""
+    lens = [300, 300, 17]
+    k = torch.full((617, D), size * 6 / 7)
+    best = [0, 300 + 299, 600 + 16]
+    k[best] = size
+    c = Cache(k, normal((617, D), 11), lens, cuda_device)
+    q = torch.full((3, 4, D), size).half() if size < 6e4 else torch.full((3, 4, D), size).bfloat16()
+    got = c.kv.decode(q.to(cuda_device), 1.0)
+    for b in range(3):
+        want = c.rows(b)[1][best[b] - sum(lens[:b])].expand(4, D)
+        close(got[b], want, want.abs() * (2.0 ** -11 + 2.0 ** -14) + c.rows(b)[2][0] * 2.0 ** -13 + half_step(want, torch.bfloat16))
