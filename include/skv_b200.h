@@ -212,8 +212,8 @@ int skv_rope_quant_append(const void* qkv, int qkv_is_bf16, void* q_out, void* k
  * copied.  freqs: device array of rotary_dim / 2 uint64, round(f_i / (2 pi) * 2^64): the angle at any position is exact to
  * the rounding of f_i.  dtype: 0 fp16, 1 bf16, 2 fp32 (q, k and outputs alike; arithmetic in fp32).  positions: int32, or
  * int64 with positions_are_64.  Strides in elements, channels contiguous; an output may be its input (then channels
- * behind rotary_dim are not touched), not overlap it otherwise, and rows of the outputs must not share memory (strides
- * below D, or one destination for q and k, are refused).  Hq or Hk may be 0 with null pointers.  rotary_dim even. */
+ * behind rotary_dim are not touched), not overlap it otherwise, and rows of the outputs must not share memory, nor a row of
+ * q_out with one of k_out (refused; so are q_out and k_out that reach into one another with different token strides).  Hq or Hk may be 0 with null pointers.  rotary_dim even. */
 int skv_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, const void* positions,
                int positions_are_64, const unsigned long long* freqs, int T, int Hq, int Hk, int D,
                int rotary_dim, int interleaved, double rope_factor, int adjoint,

@@ -211,6 +211,39 @@ __global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) 
     }
 }
 
+static long long magnitude(long long x) { return x < 0 ? -x : x; }
+
+// Whether two of the rows i * a + j * b (i < n, j < m), `width` long, share memory.
+static bool rows_share(long long n, long long m, long long a, long long b, long long width) {
+    a = magnitude(a); b = magnitude(b);                 // (counting i or j from the other end changes no distance)
+    if ((n > 1 && a < width) || (m > 1 && b < width)) return true;
+    if (n <= 1 || m <= 1 || b >= (n - 1) * a + width || a >= (m - 1) * b + width) return false;
+    for (long long j = 1; j < m; ++j)                   // neither lies whole in a step of the other: the nearest steps of i to j's
+        for (long long i = j * b / a; i <= j * b / a + 1; ++i)
+            if (i < n && magnitude(i * a - j * b) < width) return true;
+    return false;
+}
+
+// The same for a row of q (i * aq + j * bq, j < Hq) and one of k (delta + i * ak + j * bk, j < Hk).  Views whose spans meet are
+// looked into where they have one token stride; others count as sharing.
+static bool views_share(long long T, long long Hq, long long aq, long long bq, long long Hk, long long ak, long long bk,
+                        long long delta, long long width) {
+    auto low = [](long long n, long long s) { return s < 0 ? (n - 1) * s : 0; };
+    auto high = [](long long n, long long s) { return s > 0 ? (n - 1) * s : 0; };
+    const long long q0 = low(Hq, bq), q1 = high(Hq, bq) + width, k0 = delta + low(Hk, bk), k1 = delta + high(Hk, bk) + width;
+    if (q0 + low(T, aq) >= k1 + high(T, ak) || k0 + low(T, ak) >= q1 + high(T, aq)) return false;
+    if (T > 1 && aq != ak) return true;
+    const long long a = T > 1 ? magnitude(aq) : 0;
+    const bool apart = q0 >= k1 || k0 >= q1;            // within a token
+    if (apart && (a == 0 || (q1 > k1 ? q1 : k1) - (q0 < k0 ? q0 : k0) <= a)) return false;
+    for (long long j = 0; j < Hq; ++j)
+        for (long long k = 0; k < Hk; ++k) {
+            const long long x = magnitude(delta + k * bk - j * bq), i = a ? x / a : 0;
+            if ((i < T && x - i * a < width) || (a && i + 1 < T && (i + 1) * a - x < width)) return true;
+        }
+    return false;
+}
+
 template <typename T, int E, bool INTER>
 static int launch(Params& p, int tail, cudaStream_t st) {
     constexpr int NP = INTER ? E / 2 : E, U = INTER ? 8 : 4;
@@ -265,13 +298,11 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
         return fail(SKV_ERR_BAD_ARG, "skv_rotary: rotary_dim %d must be even and in 2..%d", rotary_dim, D);
     if (dtype < 0 || dtype > 2) return fail(SKV_ERR_UNSUPPORTED, "skv_rotary: dtype %d is not fp16, bf16 or fp32", dtype);
     // Rows that share memory would be turned by several threads at once: views with a repeated or shortened stride as
-    // destination (an expanded tensor rotated in place), or one destination for both.
-    auto overlaps = [&](int H, long long dt, long long dh) {
-        const long long a = dt < 0 ? -dt : dt, b = dh < 0 ? -dh : dh;
-        return (T > 1 && a < D) || (H > 1 && b < D) || (T > 1 && H > 1 && a == b);
-    };
-    if ((Hq && overlaps(Hq, q_out_stride_t, q_out_stride_h)) || (Hk && overlaps(Hk, k_out_stride_t, k_out_stride_h)) ||
-        (Hq && Hk && q_out == k_out))
+    // destination (an expanded or sliding view rotated in place), or heads that q and k have in common.
+    const long long esz = dtype == 2 ? 4 : 2;
+    if ((Hq && rot::rows_share(T, Hq, q_out_stride_t, q_out_stride_h, D)) || (Hk && rot::rows_share(T, Hk, k_out_stride_t, k_out_stride_h, D)) ||
+        (Hq && Hk && rot::views_share(T, Hq, q_out_stride_t * esz, q_out_stride_h * esz, Hk, k_out_stride_t * esz, k_out_stride_h * esz,
+                                      static_cast<const char*>(k_out) - static_cast<const char*>(q_out), D * esz)))
         return fail(SKV_ERR_BAD_ARG, "skv_rotary: rows of the outputs overlap");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(SKV_ERR_CUDA, "cannot switch to device %d", device);
@@ -286,8 +317,7 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
 
     // The widest vector that the row's parts and every pointer and stride allow: 16 bytes where a layout is an ordinary one,
     // down to single elements for odd rotary widths or views (interleaved: to pairs, fetched one by one).
-    const int esz = dtype == 2 ? 4 : 2;
-    int vec = 16 / esz;
+    int vec = 16 / (int)esz;
     bool same = true;   // nothing behind the rotated part to copy when a row is rotated in place
     for (int w = 0; w < 2; ++w) {
         if (!(w ? Hk : Hq)) continue;
