@@ -30,7 +30,8 @@ def frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> t
     * ``"llama3"``: pairs that turn more than ``high_freq_factor`` times over ``original_max_position`` tokens are kept, those
       that turn less than ``low_freq_factor`` times divided by ``factor``, those between blended;
     * ``"yarn"``: a ramp over the pairs between ``beta_fast`` (32) and ``beta_slow`` (1) turns over
-      ``original_max_position`` tokens, and values multiplied by ``attention_factor`` (``0.1 ln(factor) + 1``).
+      ``original_max_position`` tokens, and values multiplied by ``attention_factor`` (``0.1 ln(factor) + 1``, 1 for factors
+      up to 1).
     """
     R = rotary_dim
     if not theta > 1.0 or not math.isfinite(theta):
@@ -67,7 +68,7 @@ def frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> t
         high = min(math.ceil(pair(scaling.get("beta_slow") or 1.0)), R - 1)
         width = max(high - low, 0.001)
         ramp = [min(1.0, max(0.0, (i - low) / width)) for i in range(R // 2)]
-        factor = scaling.get("attention_factor") or 0.1 * math.log(scaling["factor"]) + 1.0
+        factor = scaling.get("attention_factor") or 0.1 * math.log(max(scaling["factor"], 1.0)) + 1.0
         return [x / scaling["factor"] * r + x * (1 - r) for x, r in zip(f, ramp)], factor
     return f, 1.0
 
