@@ -44,7 +44,11 @@ def frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> t
         need, may = _SCALING_KEYS[kind], _SCALING_OPTIONAL.get(kind, set())
         if not need <= given or not given <= need | may:
             raise RuntimeError(f"rope scaling {kind!r} takes {sorted(need)} and may take {sorted(may)}, got {sorted(given)}")
-        if any(not (float(scaling[k]) > 0.0 and math.isfinite(float(scaling[k]))) for k in given if scaling[k] is not None):
+        try:   # (an optional value that is None counts as not given)
+            scaling = {k: float(scaling[k]) for k in given if scaling[k] is not None or k in need}
+        except (TypeError, ValueError) as e:
+            raise RuntimeError(f"rope scaling values must be numbers: {e}") from None
+        if any(not (v > 0.0 and math.isfinite(v)) for v in scaling.values()):
             raise RuntimeError("rope scaling values must be positive and finite")
     if kind == "ntk" and R > 2:
         theta = theta * scaling["factor"] ** (R / (R - 2))
