@@ -390,7 +390,7 @@ class DecodeModel:
         from . import _C
         sh, D, B = self.shard, self.cfg.D, qkv.shape[0]
         sparse = self.layer_modes[li] == "quest"
-        a = torch.empty((B, sh.n_q, D), dtype=dtype, device=qkv.device)
+        a = None if sparse else torch.empty((B, sh.n_q, D), dtype=dtype, device=qkv.device)   # (sparse layers bring their own)
         if self.rope is not None:
             q = paged.append_tokens(qkv, self._layer_kv(cache, pos), sh.n_q, self.rope, cu_new=cu, status=self.status)
             if cache.k_bits == 4:

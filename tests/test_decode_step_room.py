@@ -134,3 +134,18 @@ def test_steps_past_a_sequences_own_pages(cuda_device, clean_words, bits, fused,
         assert (c.buf != old).flatten(1).any(1).nonzero().flatten().tolist() == [int(m.page_table[1, 1])]
     with pytest.raises(RuntimeError, match=r"\[0\]"):
         m.check_cache()
+
+
+@pytest.mark.gpu
+def test_sparse_layers_allocate_no_dense_output(cuda_device, monkeypatch):
+    """A block-sparse layer's attention brings its own output; a dense one's is allocated for it."""
+    cfg = ds.ModelConfig(layers=2, hidden=512, Hq=8, Hkv=2, D=128, mlp=1024, vocab=512)
+    m = ds.DecodeModel(cfg, shard_heads(8, 2, 1, 0), cuda_device, dtype=torch.bfloat16, layer_modes=["quest", "dense"])
+    m.init_cache(torch.tensor([200, 90], dtype=torch.int32))
+    made, real = [], torch.empty
+    monkeypatch.setattr(ds.torch, "empty", lambda *a, **k: made.append((a[0], k.get("dtype"))) or real(*a, **k))
+    for li in range(2):
+        made.clear()
+        qkv = torch.zeros(2, 12 * 128, dtype=torch.bfloat16, device=cuda_device)
+        m._fused_attention(li, qkv, m.caches[li], m.seq_lens, m.seq_lens + 1, 0.1, torch.bfloat16)
+        assert made.count(((2, 8, 128), torch.bfloat16)) == li
