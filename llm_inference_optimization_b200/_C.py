@@ -254,6 +254,9 @@ def fused_gqa_paged(Q: Tensor, k_pool: Tensor, v_pool: Tensor, k_scale: Tensor, 
     return out
 
 
+_KV4_LONGEST = 2 ** 31 - 17   # tokens of a sequence that the kernel's 32-bit positions hold
+
+
 def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: Tensor | None, scale: float, *,
                   cu_q: Tensor | None = None, max_seq_len: int | None = None, out: Tensor | None = None,
                   status: Tensor | None = None) -> Tensor:
@@ -299,8 +302,9 @@ def fused_gqa_kv4(Q: Tensor, pool: Tensor, page_table: Tensor | None, seq_lens: 
         _require(seq_lens.dtype is torch.int32 and seq_lens.shape == (B,) and seq_lens.is_contiguous()
                  and seq_lens.device == dev, "seq_lens must be a contiguous int32 [B] tensor on Q's device")
         lens = seq_lens.data_ptr()
-    N = int(max_seq_len) if max_seq_len is not None else max_pages * 16
-    _require(0 < N <= max_pages * 16, "max_seq_len must be in (0, max_pages * 16]")
+    room = min(max_pages * 16, _KV4_LONGEST)
+    N = int(max_seq_len) if max_seq_len is not None else room
+    _require(0 < N <= room, "max_seq_len must be in (0, max_pages * 16] and below 2^31 - 16")
     if out is None:
         out, out_bf16 = torch.empty_like(Q), bf16
     else:
