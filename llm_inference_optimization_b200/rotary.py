@@ -135,4 +135,6 @@ class RotaryEmbedding:
                 dev.index, _workspace.stream(dev.index))
             if rc:
                 _lib.check(rc, "rotary")
+        if inplace:   # autograd then refuses a backward pass that needs the rows as they were
+            torch.autograd.graph.increment_version(q if k is None else (q, k))
         return qo if k is None else (qo, ko)
