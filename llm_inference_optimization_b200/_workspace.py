@@ -34,13 +34,21 @@ def stream(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+def _capturing(index: int) -> bool:
+    """Whether the current stream of device ``index``, which need not be the current device, is being captured."""
+    if torch.cuda.current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def scratch(kind: str, nbytes: int, head: int, device: torch.device, handle: int) -> torch.Tensor:
     """Like :func:`get` for kernels of which only the first ``head`` bytes must be zero, and safe under graph capture.
 
     ``device`` has an index, ``handle`` is its current stream (:func:`stream`).  A call that is being captured gets a buffer
     of the graph's own, whose head is cleared by a node of the graph: two graphs, or a graph and eager calls, never share
     one, however their replays overlap."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(device.index):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:head].zero_()
         return buf
