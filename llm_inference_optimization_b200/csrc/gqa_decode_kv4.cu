@@ -107,6 +107,7 @@ struct Seq {
 template <int NC>
 __device__ __forceinline__ Seq sequence(const Params& p, int b) {
     Seq s;
+    b = SKV_INDEX(b, p.B);
     s.q0 = p.cu_q ? min(max(p.cu_q[b], 0), p.T) : b;
     s.nq = p.cu_q ? min(max(p.cu_q[b + 1], s.q0), p.T) - s.q0 : 1;
     s.len = p.seq_lens ? min(max(p.seq_lens[b], 0), p.N) : p.N;
@@ -192,7 +193,7 @@ __device__ __forceinline__ constexpr float exp2_of(int e) {
 // Column `col` of the item's list (query token col / G, head col % G), channels d .. d + 3
 __device__ __forceinline__ void store_out(const Params& p, const Segment& x, int D, int col, int d, float4 v, float L) {
     const float inv = L == 0.f ? 0.f : 1.f / L;        // nothing visible: zeros; a NaN stays one
-    const long long at = ((long long)(x.s.q0 + col / p.G) * p.Hq + x.h * p.G + col % p.G) * D + d;
+    const long long at = ((long long)SKV_INDEX(x.s.q0 + col / p.G, p.T) * p.Hq + SKV_INDEX(x.h * p.G + col % p.G, p.Hq)) * D + SKV_INDEX(d, D - 3);
     uint2 r;
     if (p.out_bf16) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv), b = __floats2bfloat162_rn(v.z * inv, v.w * inv);
@@ -219,7 +220,7 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
     // the k-th partial row of thread i: the same for all but the first CTA, whose slot is its second
     auto row = [&](int i, int k) {
         const int pos = i % places;
-        const long long slot = 2ll * (x.c_first + k) + (k == 0 ? 1 : 0);
+        const long long slot = 2ll * SKV_INDEX(x.c_first + k, (int)gridDim.x) + (k == 0 ? 1 : 0);
         return p.partial_o + (slot * NC + pos / (D / 4)) * D + pos % (D / 4) * 4;
     };
     float4 v[U];                                        // asked for before the weights are known (past the end: the last row again)
@@ -235,7 +236,7 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
         for (int i = 0; i < REGS; ++i) {
             const int k = lane + 32 * i;
             ml[i] = make_float2(-INFINITY, 0.f);
-            if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + ((2ll * (x.c_first + k) + (k == 0 ? 1 : 0)) * NC + c) * 2));
+            if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + ((2ll * SKV_INDEX(x.c_first + k, (int)gridDim.x) + (k == 0 ? 1 : 0)) * NC + c) * 2));
         }
 #pragma unroll
         for (int i = 0; i < REGS; ++i) M = fmaxf(M, ml[i].x);
@@ -246,7 +247,7 @@ __device__ __forceinline__ void combine(const Params& p, const Segment& x, int n
             const int k = lane + 32 * i;
             if (k < n) {
                 const float w = fast_exp2(ml[i].x - M);
-                weight[k * cols + c] = w;
+                weight[SKV_INDEX(k * cols + c, MAX_GRID * NC)] = w;
                 L = fmaf(ml[i].y, w, L);
             }
         }
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
     auto load_page = [&](int r) {
         int page = 0;
         if (r < rec_end)
-            page = p.page_table ? __ldg(p.page_table + (long long)seq * p.max_pages + r) : seq * p.max_pages + r;
+            page = p.page_table ? __ldg(p.page_table + (long long)SKV_INDEX(seq, p.B) * p.max_pages + SKV_INDEX(r, p.max_pages)) : seq * p.max_pages + r;
         return checked_page(page, p.num_pages, bad_page);
     };
     auto issue = [&](int k, auto certain_constant) {  // (certain: the caller knows that record k exists)
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
         const int page = __shfl_sync(0xffffffffu, page_now, k & 31);
         if (CERTAIN || k < n_rec) {
             const uint8_t* src = head_base + (unsigned long long)(uint32_t)SKV_INDEX(page, p.num_pages) * p.sp;
-            const uint32_t dst = ring + in_off + lane * 16;
+            const uint32_t dst = ring + SKV_INDEX(in_off, (STAGES - 1) * REC + 1) + lane * 16;
 #pragma unroll
             for (int i = 0; i < REC / 512; ++i) cp_async16(dst + i * 512, src + i * 512);
             cp_async16_if(dst + REC / 512 * 512, src + REC / 512 * 512, lane < REC % 512 / 16);
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
         if (warp < NT) {
             const int c = x.chunk * NC + warp * 8 + g;
             const bool in = c < total_cols;
-            const long long row = in ? ((long long)(x.s.q0 + c / p.G) * p.Hq + x.h * p.G + c % p.G) * D : 0;
+            const long long row = in ? ((long long)SKV_INDEX(x.s.q0 + c / p.G, p.T) * p.Hq + SKV_INDEX(x.h * p.G + c % p.G, p.Hq)) * D : 0;
 #pragma unroll
             for (int w = 0; w < W; ++w)
                 cp_async16_or_zero(smem_u32(q_to) + ((warp * W + w) * 32 + lane) * 16, static_cast<const __half*>(p.q) + row + w * 32 + tq * 8, in);
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
             cp_async_wait<STAGES - 2>();
             __syncwarp();                              // record k is here, and every lane is done with record k - 1
             issue(k + STAGES - 1, Constant<!MASKED>{});
-            const uint32_t rec = ring + out_off;
+            const uint32_t rec = ring + SKV_INDEX(out_off, (STAGES - 1) * REC + 1);
             out_off = out_off == (STAGES - 1) * REC ? 0 : out_off + REC;
             const int t0 = (r_first + k * NW) * 16 + tok_a;   // this lane's tokens: t0, t0 + 2
             auto hidden = [&](int j, int nt) { return t0 + (j & 2) >= limit[nt][j & 1]; };
@@ -784,10 +785,10 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
         const int col0 = done.chunk * NC, cols = min(done.s.nq * p.G - col0, NC);
 
         // ---- merge the warps
-        const long long slot = 2ll * blockIdx.x + (done.r0 == 0 ? 1 : 0);
+        const long long slot = SKV_INDEX(2 * (int)blockIdx.x + (done.r0 == 0 ? 1 : 0), 2 * MAX_GRID);
         __syncthreads();
         for (int i = threadIdx.x; i < cols * (D / 4); i += THREADS) {
-            const int c = i / (D / 4), d = i % (D / 4) * 4;
+            const int c = SKV_INDEX(i / (D / 4), NC), d = i % (D / 4) * 4;
             float2 ml[NW];
             float M = -INFINITY;
 #pragma unroll
@@ -820,8 +821,9 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
-                const int last = atomicAdd(&p.tickets[done.c_first], 1) == n - 1;
-                if (last) p.tickets[done.c_first] = 0;  // ready for the next launch on this workspace
+                int* ticket = p.tickets + SKV_INDEX(done.c_first, (int)gridDim.x);
+                const int last = atomicAdd(ticket, 1) == n - 1;
+                if (last) *ticket = 0;                 // ready for the next launch on this workspace
                 state->last = last;
             }
             __syncthreads();

@@ -63,7 +63,7 @@ template <int LPR>
 __device__ __forceinline__ int sequence_of(const int* cu, int B, long long t, int l, unsigned group) {
     if (B <= 16 * LPR) {
         int n = 0;
-        for (int i = l; i < B; i += LPR) n += cu[i + 1] <= t;
+        for (int i = l; i < B; i += LPR) n += cu[SKV_INDEX(i, B) + 1] <= t;
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) n += __shfl_xor_sync(group, n, o);
         return n;
@@ -71,7 +71,7 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, long long t, in
     int lo = 0, hi = B;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
+        if (cu[SKV_INDEX(mid, B) + 1] <= t) lo = mid + 1; else hi = mid;
     }
     return lo;
 }
@@ -216,7 +216,8 @@ __device__ __forceinline__ int page_of(const Pools& c, int b, long long pos, int
     if (pos < 0 || pos >= (long long)c.max_pages * c.page_size) return -1;
     const int lp = (int)(pos / c.page_size);
     slot = (int)(pos - (long long)lp * c.page_size);
-    const int page = c.page_table ? c.page_table[(long long)b * c.max_pages + lp] : b * c.max_pages + lp;
+    const int page = c.page_table ? c.page_table[(long long)b * c.max_pages + SKV_INDEX(lp, c.max_pages)] : b * c.max_pages + lp;
+    slot = SKV_INDEX(slot, c.page_size);
     if ((unsigned)page >= (unsigned)c.num_pages) {
         if (c.status) atomicOr(c.status, SKV_DEV_BAD_PAGE);
         return -1;
@@ -248,11 +249,11 @@ __global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendP
     const int d0 = l * 8;
 
     // rows are asked for before anything is known of their sequence (one behind the last reads the first row and drops it)
-    const T* src = static_cast<const T*>(p.qkv) + (in ? t : 0) * p.qkv_stride + d0;
+    const T* src = static_cast<const T*>(p.qkv) + (long long)SKV_INDEX(in ? t : 0, p.T) * p.qkv_stride + d0;
     uint4 next[U];
     auto load = [&](int h0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = ld_stream16(src + (long long)min(h0 + u * WARPS, heads - 1) * D);
+        for (int u = 0; u < U; ++u) next[u] = ld_stream16(src + (long long)SKV_INDEX(min(h0 + u * WARPS, heads - 1), heads) * D);
     };
     load(h_begin);
 
@@ -265,14 +266,16 @@ __global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendP
     int page = -1, slot = 0;
     bool mine = b < p.B;                     // rows before the first sequence and behind the last are left alone
     if (mine) {
+        b = SKV_INDEX(b, p.B);
         const long long i = p.cu_new ? t - p.cu_new[b] : 0;
         mine = i >= 0;
         pos = (long long)p.seq_lens[b] + i;
     }
     if (mine) {
         page = page_of(p.c, b, pos, slot);
-        if (p.positions) pos = p.pos64 ? static_cast<const long long*>(p.positions)[t]
-                                       : (long long)static_cast<const int*>(p.positions)[t];
+        const int at = SKV_INDEX(t, p.T);
+        if (p.positions) pos = p.pos64 ? static_cast<const long long*>(p.positions)[at]
+                                       : (long long)static_cast<const int*>(p.positions)[at];
     }
 
     // the lane's channels: 8 pairs with a partner lane (half layout; the first half takes the sine negative), or 4 of its own
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 6) append_tokens_kernel(const AppendP
         for (int i0 = 0; i0 < ROWS * half; i0 += THREADS) {
             const int i = min(i0 + (int)threadIdx.x, ROWS * half - 1), r = i / half;
             const long long at = __shfl_sync(group, pos, r * LPR);
-            table[i] = rotary_cos_sin(at, p.freqs[i - r * half], p.factor);
+            table[SKV_INDEX(i, ROWS * D / 2)] = rotary_cos_sin(at, p.freqs[SKV_INDEX(i - r * half, half)], p.factor);
         }
         __syncthreads();
         if (turned) {
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(THREADS) read_tokens_kernel(const ReadParams p
     const long long t = (long long)(warp / (unsigned)p.head_splits) * (32 / LPR) + lane / LPR;
     const bool in = t < p.T;
     const int s = sequence_of<LPR>(p.cu, p.B, in ? t : (long long)p.T, l, 0xffffffffu);
-    if (!in || s >= p.B || t < p.cu[s]) return;   // rows before the first sequence and behind the last are left alone
+    if (!in || s >= p.B || t < p.cu[SKV_INDEX(s, p.B)]) return;   // rows before the first sequence and behind the last are left alone
     int slot = 0;
     const long long pos = (p.starts ? p.starts[s] : 0) + (t - p.cu[s]);
     const int page = page_of(p.c, s, pos, slot);
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(THREADS) read_tokens_kernel(const ReadParams p
             else
                 decode8<CACHE>(*reinterpret_cast<const uint2*>(p.c.v + pg * p.c.sp + h * p.c.sh + slot * p.c.ss + l * 8), vs, v);
         }
-        const long long o = (t * p.Hkv + h) * D + l * 8;
+        const long long o = ((long long)SKV_INDEX(t, p.T) * p.Hkv + SKV_INDEX(h, p.Hkv)) * D + l * 8;
         const bool bf = p.out_bf16;
         uint4 a = make_uint4(pack16(k[0], k[1], bf), pack16(k[2], k[3], bf), pack16(k[4], k[5], bf), pack16(k[6], k[7], bf));
         uint4 c = make_uint4(pack16(v[0], v[1], bf), pack16(v[2], v[3], bf), pack16(v[4], v[5], bf), pack16(v[6], v[7], bf));

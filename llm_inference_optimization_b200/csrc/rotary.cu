@@ -115,12 +115,12 @@ __global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) 
     const int first = threadIdx.x % p.width, rest = threadIdx.x / p.width;
     const int lane = rest % p.lanes, tt = rest / p.lanes;
     const bool live = tt < nt;
-    const long long t = t0 + (live ? tt : 0);
+    const long long t = SKV_INDEX(t0 + (live ? tt : 0), p.T);
 
     V a[U], b[U];
     auto channel = [&](int u) { return u < p.turn_units ? u * E : p.R + (u - p.turn_units) * E; };
     auto load = [&](int u, int h0) {
-        const int c = channel(u);
+        const int c = SKV_INDEX(channel(u), p.D - (LOOSE ? 0 : E - 1));
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int h = min(h0 + k * p.lanes, p.H - 1), w = h >= p.Hq;   // (past the last head: that one again, not stored)
@@ -137,15 +137,15 @@ __global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) 
     // the block's angles: what they need is asked for first, then the rows, and the sines are worked out while those come
     const int pairs = p.turn_units * NP, angles = nt * pairs;
     auto angle = [&](int i, long long& pos, unsigned long long& f) {
-        const int x = i / pairs;
-        pos = p.pos64 ? static_cast<const long long*>(p.positions)[t0 + x] : (long long)static_cast<const int*>(p.positions)[t0 + x];
-        f = p.freqs[i - x * pairs];
+        const int x = i / pairs, t = SKV_INDEX(t0 + x, p.T);
+        pos = p.pos64 ? static_cast<const long long*>(p.positions)[t] : (long long)static_cast<const int*>(p.positions)[t];
+        f = p.freqs[SKV_INDEX(i - x * pairs, p.R / 2)];
     };
     auto write = [&](int i, long long pos, unsigned long long f) {
         const int x = i / pairs, r = i - x * pairs;
         float2 cs = rotary_cos_sin(pos, f, p.factor);
         cs.y *= p.sign;
-        table[(x * NP + r % NP) * p.turn_units + r / NP] = cs;
+        table[SKV_INDEX((x * NP + r % NP) * p.turn_units + r / NP, p.tokens * NP * p.turn_units)] = cs;
     };
     {
         long long pos = 0;
@@ -166,12 +166,12 @@ __global__ void __launch_bounds__(MAX_THREADS, 4) rotary_kernel(const Params p) 
         if (turned) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const float2 f = table[(tt * NP + i) * p.turn_units + u];
+                const float2 f = table[SKV_INDEX((tt * NP + i) * p.turn_units + u, p.tokens * NP * p.turn_units)];
                 cs[i] = f.x;
                 sn[i] = f.y;
             }
         }
-        const int c = channel(u);
+        const int c = SKV_INDEX(channel(u), p.D - (LOOSE ? 0 : E - 1));
         for (int h0 = lane; h0 < p.H; h0 += U * p.lanes) {
             if (u != first || h0 != lane) load(u, h0);
 #pragma unroll
@@ -335,3 +335,5 @@ extern "C" int skv_rotary(const void* q, const void* k, void* q_out, void* k_out
     if (dtype == 1) return rot::launch_vec<__nv_bfloat16>(vec, p, tail, interleaved, st);
     return rot::launch_vec<float>(vec, p, tail, interleaved, st);
 }
+
+SKV_BOUNDS_GETTER(skv_debug_bounds_rotary)
