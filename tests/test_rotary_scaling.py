@@ -26,3 +26,18 @@ def test_values_that_are_no_numbers_are_refused(scaling):
 def test_optional_values_may_be_none():
     sc = {"type": "yarn", "factor": 4.0, "original_max_position": 4096}
     assert rotary.frequencies(64, 10000.0, sc | {"beta_fast": None, "attention_factor": None}) == rotary.frequencies(64, 10000.0, sc)
+
+
+@pytest.mark.parametrize("theta,dim", [(10000.0, 64), (500000.0, 128), (1e6, 80)])
+def test_fixed_point_frequencies_are_off_by_their_rounding(theta, dim):
+    """Against 60 digits: 2^-51 of the frequency (four roundings of 2^-53: the power, 2 pi, its product, the quotient) and half a unit of
+    the 64-bit fraction.  That, times the position, is what an angle is off by."""
+    from decimal import Decimal, localcontext
+    r = rotary.RotaryEmbedding(dim, theta, device="cpu")
+    with localcontext() as c:
+        c.prec = 60
+        pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        for i, t in enumerate(r.turns.tolist()):
+            true = (Decimal(theta).ln() * Decimal(-2 * i) / Decimal(dim)).exp() / (2 * pi)
+            off = abs(Decimal(t % (1 << 64)) / Decimal(2) ** 64 - true)
+            assert off <= true * Decimal(2) ** -51 + Decimal(2) ** -65
