@@ -513,8 +513,8 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
             }
             q_words[(nt * 3 + 0) * 32 + lane] = b0;
             q_words[(nt * 3 + 1) * 32 + lane] = b1;
-            q_words[(nt * 3 + 2) * 32 + lane] =         // 2^20 / up, and the softmax scale
-                __float_as_uint(p.scale_log2 * __uint_as_float((uint32_t)min(max(e + 137, 1), 254) << 23));
+            q_words[(nt * 3 + 2) * 32 + lane] =         // 2^20 / up, which may pass fp32's range by itself, and the softmax scale
+                __float_as_uint(p.scale_log2 * __uint_as_float((uint32_t)(e + 121) << 23) * 65536.f);
         }
         __syncthreads();
         uint32_t qbias[NT][2];

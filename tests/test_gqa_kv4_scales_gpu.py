@@ -115,3 +115,11 @@ def test_the_largest_of_large_scores_takes_all(cuda_device, D, size):
     for b in range(3):
         want = c.rows(b)[1][best[b] - sum(lens[:b])].expand(4, D)
         close(got[b], want, want.abs() * (2.0 ** -11 + 2.0 ** -14) + c.rows(b)[2][0] * 2.0 ** -13 + half_step(want, torch.bfloat16))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [-110, 100, 116, 118, 121, 124])
+def test_queries_near_the_ends_of_the_range(cuda_device, D, power):
+    """bf16 queries of 2^-110 to 2^125 with a softmax scale that keeps the scores ordinary."""
+    q = (normal((2, 8, D), 12).clamp(-3, 3) * 2.0 ** power).bfloat16()
+    Cache(normal((133, D), 13), normal((133, D), 14), [100, 33], cuda_device).check(q, D ** -0.5 * 2.0 ** -power, cuda_device, torch.bfloat16)
