@@ -629,25 +629,23 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                 uint32_t ra[W], rb[W];
                 lds<D / 8>(rec + 16 * D + g * (D / 8), ra);
                 lds<D / 8>(rec + 17 * D + g * (D / 8), rb);
+                unsigned e[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const int half = (w & 1) * 16;
+                    const uint32_t xa = MASKED && t0 >= end_tok ? 0u : ra[W / 2 + (w >> 1)] >> half & 0xffffu;
+                    const uint32_t xb = MASKED && t0 + 2 >= end_tok ? 0u : rb[W / 2 + (w >> 1)] >> half & 0xffffu;
+                    e[w] = max(xa < 0x7f80u ? xa >> 7 : 0u, xb < 0x7f80u ? xb >> 7 : 0u);
+                }
+#pragma unroll
+                for (int w = 0; w < W; ++w) e[w] = __reduce_max_sync(0xffffffffu, e[w]);   // (one behind the other, no branch between)
+                float fall[W];                         // what O of a group that grows is multiplied by, exactly while nothing underflows
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const int half = (w & 1) * 16, old = exponent_of(vdown, w);
-                    const uint32_t xa = MASKED && t0 >= end_tok ? 0u : ra[W / 2 + (w >> 1)] >> half & 0xffffu;
-                    const uint32_t xb = MASKED && t0 + 2 >= end_tok ? 0u : rb[W / 2 + (w >> 1)] >> half & 0xffffu;
-                    int e = old;
-                    if (xa < 0x7f80u) e = max(e, (int)(xa >> 7));
-                    if (xb < 0x7f80u) e = max(e, (int)(xb >> 7));
-                    e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e);
-                    if (e > old && old < 253) {        // (the same for all lanes)
-                        // O of the group moves to the new power of two, exactly while it does not underflow
-                        e = min(e + SCALE_ROOM, 253);
-                        const float c = e - old < 127 ? __uint_as_float((uint32_t)(127 - e + old) << 23) : 0.f;
-                        vdown[w >> 1] = (vdown[w >> 1] & (0xffff0000u >> half)) | (uint32_t)(254 - e) << (7 + half);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) { o[nt][2 * w][j] *= c; o[nt][2 * w + 1][j] *= c; }
-                    }
+                    const int now = (int)e[w] > old ? min((int)e[w] + SCALE_ROOM, 253) : old;
+                    fall[w] = now - old < 127 ? __uint_as_float((uint32_t)(127 - now + old) << 23) : 0.f;
+                    vdown[w >> 1] = (vdown[w >> 1] & (0xffff0000u >> half)) | (uint32_t)(254 - now) << (7 + half);
                 }
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i) {
@@ -674,20 +672,21 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                             sx = fmaxf(sx, __shfl_xor_sync(0xffffffffu, sx, x));
                             tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
                         }
+                        float c = 1.f;
                         if (tx > WEIGHT_MAX) {         // (the same for all lanes of a column)
                             const float moved = __fsub_ru(sx, WEIGHT_AIM);
                             if (fabsf(moved) >= BIG_SCORE) big = MOVE;
-                            const float c = fast_exp2(ref[nt][j] - moved);
+                            c = fast_exp2(ref[nt][j] - moved);
                             ref[nt][j] = moved;
                             lrun[nt][j] *= c;
-#pragma unroll
-                            for (int i = 0; i < 2 * W; ++i) { o[nt][i][j] *= c; o[nt][i][j + 2] *= c; }
 #pragma unroll
                             for (int i = j; i < 4; i += 2) {
                                 t[nt][i] = big ? __fsub_rn(__fmul_rn(s[nt][i], factor[nt][j]), moved) : fmaf(s[nt][i], factor[nt][j], -moved);
                                 if (MASKED && hidden(i, nt)) t[nt][i] = -INFINITY;
                             }
                         }
+#pragma unroll
+                        for (int i = 0; i < 2 * W; ++i) { o[nt][i][j] *= c * fall[i >> 1]; o[nt][i][j + 2] *= c * fall[i >> 1]; }
                     }
             }
 #pragma unroll
@@ -756,10 +755,11 @@ __global__ void __launch_bounds__((Shape<D, NT>::THREADS), 1) gqa_decode_kv4_ker
                     const int e = exponent_of(vdown, w);
                     const float up = __uint_as_float(e ? (uint32_t)e << 23 : 0x400000u);   // 2^(e - 127)
                     float4 v;
-                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * exp2_of(24 + SUMS_DOWN) * up;
-                    v.y = o[nt][2 * w][j + 2] * exp2_of(20 + SUMS_DOWN) * up;
-                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * exp2_of(24 + SUMS_DOWN) * up;
-                    v.w = o[nt][2 * w + 1][j + 2] * exp2_of(20 + SUMS_DOWN) * up;
+                    const float odd = up * exp2_of(20 + SUMS_DOWN), even = up * exp2_of(24 + SUMS_DOWN);
+                    v.x = (o[nt][2 * w][j] - o[nt][2 * w][j + 2]) * even;
+                    v.y = o[nt][2 * w][j + 2] * odd;
+                    v.z = (o[nt][2 * w + 1][j] - o[nt][2 * w + 1][j + 2]) * even;
+                    v.w = o[nt][2 * w + 1][j + 2] * odd;
                     *reinterpret_cast<float4*>(merge + (warp * NC + c) * S::ROW + 32 * w + 4 * g) = v;
                 }
             }
@@ -911,7 +911,9 @@ int skv_gqa_decode_kv4(const void* q, int q_is_bf16, const void* pool, const int
     p.status = status;
     // Columns per pass over the cache, 8 or 16.  A pass of 16 takes 7/4 of one of 8, so it pays where it saves that many of the
     // mean sequence's (query token, head) pairs' passes.  Measured with 8 | 16, D = 128, us: 16 pairs of 8 sequences of 8192
-    // tokens 42.5 | 39.9, 24 pairs 57.1 | 62.0, 32 pairs 71.6 | 63.5; 512 of one of 4096 76.2 | 65.7.
+    // tokens 42.5 | 39.9, 24 pairs 57.1 | 62.0, 32 pairs 71.6 | 63.5; 512 of one of 4096 76.2 | 65.7.  It loses where the work is
+    // small (16 pairs of one sequence of 16384: 18.7 | 22.2), which the host does not see, for it does not know the lengths; and
+    // it judges by the mean, so one chunk of a prompt among single tokens may get 8.
     const long long pairs = (long long)p.G * ((T + B - 1) / B);
     const bool wide = 7 * ((pairs + 15) / 16) < 4 * ((pairs + 7) / 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

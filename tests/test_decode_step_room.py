@@ -149,3 +149,21 @@ def test_sparse_layers_allocate_no_dense_output(cuda_device, monkeypatch):
         qkv = torch.zeros(2, 12 * 128, dtype=torch.bfloat16, device=cuda_device)
         m._fused_attention(li, qkv, m.caches[li], m.seq_lens, m.seq_lens + 1, 0.1, torch.bfloat16)
         assert made.count(((2, 8, 128), torch.bfloat16)) == li
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v_bits", [8, 4])
+def test_sparse_layers_past_a_sequences_own_pages(cuda_device, clean_words, v_bits):
+    """A block-sparse layer beside a dense one: the sequence without room stores nothing, in its metadata neither."""
+    cfg = ds.ModelConfig(layers=2, hidden=512, Hq=8, Hkv=2, D=128, mlp=1024, vocab=512)
+    m = ds.DecodeModel(cfg, shard_heads(8, 2, 1, 0), cuda_device, dtype=torch.bfloat16, layer_modes=["quest", "dense"], v_bits=v_bits, quest_top_k=2)
+    m.init_cache(torch.tensor([290, 30], dtype=torch.int32), extra_tokens=16)
+    assert m.room.tolist() == [320, 48]
+    m.seq_lens.copy_(torch.tensor([290, 48]))
+    before, meta = [c.buf.clone() for c in m.caches], m.metas[0].clone()
+    m.step(torch.tensor([3, 100], device=cuda_device))
+    for c, old in zip(m.caches, before):
+        assert (c.buf != old).flatten(1).any(1).nonzero().flatten().tolist() == [int(m.page_table[0, 290 // 16])]
+    assert torch.equal(m.metas[0][1], meta[1])
+    with pytest.raises(RuntimeError, match=r"\[1\]"):
+        m.check_cache()
