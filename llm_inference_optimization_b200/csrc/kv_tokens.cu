@@ -404,9 +404,11 @@ __global__ void __launch_bounds__(THREADS) read_tokens_kernel(const ReadParams p
     const long long t = (long long)(warp / (unsigned)p.head_splits) * (32 / LPR) + lane / LPR;
     const bool in = t < p.T;
     const int s = sequence_of<LPR>(p.cu, p.B, in ? t : (long long)p.T, l, 0xffffffffu);
-    if (!in || s >= p.B || t < p.cu[SKV_INDEX(s, p.B)]) return;   // rows before the first sequence and behind the last are left alone
+    if (!in || s >= p.B) return;             // rows behind the last sequence are left alone ...
     int slot = 0;
-    const long long pos = (p.starts ? p.starts[s] : 0) + (t - p.cu[s]);
+    const int start = p.starts ? p.starts[SKV_INDEX(s, p.B)] : 0;   // (asked for with the offset, not behind it)
+    const long long i = t - p.cu[SKV_INDEX(s, p.B)], pos = start + i;
+    if (i < 0) return;                       // ... and those before the first
     const int page = page_of(p.c, s, pos, slot);
     const long long pg = page < 0 ? 0 : page;
     const int h_end = min(p.Hkv, (split + 1) * p.heads_per_split);
