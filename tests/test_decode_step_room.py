@@ -13,7 +13,7 @@ from test_decode_step_kv4 import CFG, near
 def clean_words(cuda_device):
     """The attention kernels report a missing page to their workspaces too, which later tests expect to be clean."""
     yield
-    for kind in ("gqa", "gqa_kv4"):
+    for kind in ("gqa", "gqa_kv4", "quest"):
         for ws in _workspace.all_of(kind, cuda_device):
             ws[:4].zero_()
 
