@@ -32,9 +32,10 @@
 // lengths and walks over the items in it.  An item that spans CTAs is summed by the last of them to finish (a ticket per
 // first CTA), in the order of the sequence: results do not depend on timing.
 //
-// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 63.2 us, 4.8 TB/s, 0.73 of a copy (the
-// stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 54.4 us; one of 4093 tokens
-// 11.4 us, all of it start, merge and sum.  ncu: issue slots 63 % busy, logic pipe 55 %, tensor pipe 28 %.
+// Measured (D = 128, 8 kv-heads of 4 heads, one query each): 4 sequences of 65536 tokens 64.7 us, 4.7 TB/s, 0.71 of a copy (the
+// stream alone, without the arithmetic, takes 52.5); 16 ragged sequences of 0 .. 32000 tokens 55.8 us; one of 4093 tokens
+// 12.0 us, all of it start, merge and sum.  ncu: 318 instructions a record, issue slots 63 % busy, logic pipe 55 %, tensor pipe
+// 27 %.  (A power of two for each group of 32 channels instead of one bound for all, and scores far from zero, cost 2 %.)
 #include <cuda_bf16.h>
 
 #include "skv_common.cuh"
