@@ -265,8 +265,8 @@ int skv_read_tokens(const void* k_pool, const void* v_pool, const float* k_scale
  * q, out: [T, Hq, D], fp16 or bf16 each.  cu_q int32 [B + 1]: rows cu_q[b] .. cu_q[b + 1] are the last query tokens of
  * sequence b, query i of n sees positions < seq_lens[b] - n + i + 1 (none: zeros); NULL: one query per sequence, T = B.
  * Rows before cu_q[0] and from cu_q[B] on are left alone in out.  Products of a softmax weight and a value scale are rounded to
- * fp16: 11 bits down to 2^-22 of the largest weight times the largest scale of the same 32 channels, off by at most 2^-33 of
- * that below; sums are fp32.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
+ * fp16: 11 bits down to 2^-22 of the largest weight times the largest scale of the same 32 channels (of any token of the
+ * sequence, also one that only later queries see), off by at most 2^-33 of that below; sums are fp32.  seq_lens int32 [B] or NULL (N tokens each); page_table as for
  * skv_gqa_decode_paged.  pool strides in bytes.  D = 64 or 128, any Hq / Hkv.  The result does not depend on timing.
  * A page-table entry outside [0, num_pages) reads page 0 and sets SKV_DEV_BAD_PAGE in *status (optional int32 device word;
  * NULL: the workspace's, at offset 0).  Workspace: skv_gqa_decode_kv4_workspace_bytes(D); its first 8192 bytes are zero

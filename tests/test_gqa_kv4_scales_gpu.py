@@ -123,3 +123,22 @@ def test_queries_near_the_ends_of_the_range(cuda_device, D, power):
     """bf16 queries of 2^-110 to 2^125 with a softmax scale that keeps the scores ordinary."""
     q = (normal((2, 8, D), 12).clamp(-3, 3) * 2.0 ** power).bfloat16()
     Cache(normal((133, D), 13), normal((133, D), 14), [100, 33], cuda_device).check(q, D ** -0.5 * 2.0 ** -power, cuda_device, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bits", [10, 20, 26])
+def test_a_large_token_that_only_the_last_query_sees(cuda_device, D, bits):
+    """Value scales are bounded over all tokens of the sequence: earlier queries keep to the bound that is stated with them."""
+    n, m = 100, 4
+    v = normal((n, D), 15)
+    v[n - 1] *= 2.0 ** bits
+    c = Cache(normal((n, D), 16), v, [n], cuda_device)
+    q = normal((m, 4, D), 17).half()
+    got = c.kv.decode(q.to(cuda_device), D ** -0.5, cu_q=ints(0, m).to(cuda_device), out=torch.empty(m, 4, D, dtype=torch.bfloat16, device=cuda_device))
+    k, values, step = c.rows(0)
+    want, tol = attend(q, k, values, step, D ** -0.5, m)
+    for i in range(m):
+        see = n - m + i + 1
+        p = torch.softmax(q[i].double() @ k[:see, 0].T * D ** -0.5, -1)
+        tol[i] += see * p.amax(-1)[:, None] * step[:, 0].amax(0) * (15 * 2.0 ** -33)
+    close(got, want, tol + half_step(want, torch.bfloat16))
