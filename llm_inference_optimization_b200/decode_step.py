@@ -327,7 +327,7 @@ class DecodeModel:
         """Raise if a sequence has outgrown its own pages (or a kernel met a page-table entry outside the pool).
 
         Steps and prompts never ask the host how long a sequence is: a token without a page is not stored, the others are
-        untouched, and the sequence's logits mean nothing from there on.  This waits for the device; call it between steps."""
+        untouched, and the sequence's logits mean nothing from that call on.  This waits for the device; call it between steps."""
         over = (self.seq_lens > self.room).nonzero().flatten().tolist()
         bad = int(self.status)
         self.status.zero_()

@@ -129,3 +129,57 @@ def test_rows_take_the_codes_of_torchs_quantisers(cuda_device, fmt, dtype):
                 scale = torch.where(amax > 0, amax / 127.0, torch.ones_like(amax))
                 codes = (rows.float() / scale[..., None]).round().to(torch.int8)
         assert torch.equal(held(parts[1]), scale) and torch.equal(held(parts[0]), codes)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_without_a_page_table(cuda_device, fmt):
+    """Sequence b owns pages b * max_pages and on: the same bytes as with the table that says so."""
+    size, per, B = (48 if fmt == "pools" else 16), 3, 3
+    g = torch.Generator().manual_seed(8)
+    lens, new = ints(0, size + 3, 2 * size + 1), [size + 5, 4, size]     # the last runs past its pages
+    table = torch.arange(B * per, dtype=torch.int32).view(B, per)
+    with_table, without = (empty_cache(fmt, B * per, 2, 128, table, lens, B, cuda_device) for _ in range(2))
+    without.page_table = None
+    qkv = torch.randn(sum(new), 7 * 128, generator=g).bfloat16().to(cuda_device)
+    cu = offsets(new).to(cuda_device)
+    q = [paged.append_tokens(qkv, kv, 3, cu_new=cu) for kv in (with_table, without)]
+    assert torch.equal(*q) and all(torch.equal(a, b) for a, b in zip(cache_bytes(with_table), cache_bytes(without)))
+    rows = [paged.read_tokens(kv, cu, sum(new), starts=kv.seq_lens) for kv in (with_table, without)]
+    assert all(torch.equal(a, b) for a, b in zip(*rows)) and rows[0][0][-size:].any() and not rows[0][0][-1].any()
+
+
+@pytest.mark.parametrize("fmt", ["kv4", "e4m3"])
+def test_captured_with_offsets_made_in_the_graph(cuda_device, fmt):
+    """Append and read-back captured with offsets and positions that the graph makes, replayed on changed inputs, an eager call on another
+    stream meanwhile."""
+    B, most = 40, 30
+    table, total = page_table([3] * B, 0, torch.Generator().manual_seed(9))
+    kv, other, plain = (empty_cache(fmt, total, 2, 128, table, ints(*range(B)), B, cuda_device) for _ in range(3))
+    qkv = torch.zeros(B * most, 6 * 128, dtype=torch.float16, device=cuda_device)
+    counts = torch.zeros(B, dtype=torch.int32, device=cuda_device)
+
+    def work(cache):
+        cu = torch.cat([counts[:1] * 0, counts.cumsum(0, dtype=torch.int32)])
+        q = paged.append_tokens(qkv * 2, cache, 2, cu_new=cu + 0, q_out=torch.zeros(B * most, 2, 128, dtype=torch.float16, device=cuda_device))
+        K, V = paged.read_tokens(cache, cu + 0, B * most, starts=cache.seq_lens + 0)
+        here = torch.arange(B * most, device=cuda_device) < cu[-1]
+        return q, torch.where(here[:, None, None], K, 0), torch.where(here[:, None, None], V, 0)
+
+    work(kv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(kv)
+    side = torch.cuda.Stream()
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        qkv.copy_(torch.randn(B * most, 6 * 128, generator=g))
+        counts.copy_(torch.randint(0, most + 1 - 17, (B,), generator=g, dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            mixed = work(other)
+        torch.cuda.synchronize()
+        want = work(plain)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(mixed, want))
+        assert all(torch.equal(a, b) for a, b in zip(cache_bytes(kv), cache_bytes(plain)))
